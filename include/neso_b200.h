@@ -50,6 +50,11 @@ typedef void* neso_stream_t;
 #define NESO_ERR_DEVICE_TIMEOUT (-6) /* a bounded device-side wait expired */
 #define NESO_ERR_NO_DEVICE (-7)
 
+/* Element types of the entry points that take more than one. */
+#define NESO_F16 0
+#define NESO_BF16 1
+#define NESO_F32 2
+
 /* ------------------------------------------------------------- runtime -- */
 NESO_API const char* neso_last_error_string(void);
 NESO_API int neso_version(void);
@@ -284,6 +289,104 @@ NESO_API int neso_w4a16_g128_matmul(const void* X, const uint8_t* Wq, const void
  * neso_device_status until neso_clear_device_status. */
 NESO_API int neso_w8a16_matmul_mnk_noalloc(const void* X, const int8_t* W, const void* scale, float* Y, int32_t M,
                                            int32_t N, int32_t K, neso_stream_t stream);
+
+/* ------------------------------------- one decoding step, paged cache -- */
+/* Extensions (no reference kernel): what a decoding loop runs next to the
+ * GEMV-shaped quantized matmuls. Keys and values live in pages: a cache holds
+ * [num_pages, Hkv, page_size, D] 16-bit elements, addressed through a page,
+ * head and token stride (elements; D is contiguous, everything else any
+ * multiple of 8), so views of other orders or of a joint K/V buffer work. A
+ * sequence's token t lies in page block_tables[b][t / page_size], row
+ * t % page_size. Lengths, tables, positions and slots are device data: no call
+ * reads them on the host, and a captured graph follows them. `workspace` is
+ * the caller's and belongs to the call until it has run; calls that may
+ * overlap need one each. */
+
+/* Rotate q and k of N new tokens and write k and v to the cache.
+ *   pair d < half of token n turns by row positions[a][n] of cos/sin
+ *   [table_rows, half], where a is the axis whose section holds d (sections:
+ *   `axes` host ints that add up to half; NULL for one axis):
+ *     y[d] = x[d] cos - x[d + half] sin,  y[d + half] = x[d] sin + x[d + half] cos
+ *   computed in fp32 and rounded once; elements from 2 * half on are copied.
+ * q [N, Hq, D], k, v [N, Hkv, D] with token and head strides; q_out [N, Hq, D]
+ * contiguous (may be q itself when q is contiguous). slots[n] is token n's
+ * place, page * page_size + row. A slot outside the cache marks padding: such
+ * a token is not cached and its row of q_out is zero. A position outside the
+ * table turns to NaN. Slots of one call have to differ from each other. */
+NESO_API int neso_rope_paged_append(const void* q, const void* k, const void* v, const float* cos, const float* sin,
+                                    const int32_t* positions, const int64_t* slots, void* q_out, void* k_cache,
+                                    void* v_cache, int32_t dtype, int32_t N, int32_t Hq, int32_t Hkv, int32_t D,
+                                    int32_t half, int32_t table_rows, int32_t axes, const int32_t* sections,
+                                    int64_t q_stride_n, int64_t q_stride_h, int64_t k_stride_n, int64_t k_stride_h,
+                                    int64_t v_stride_n, int64_t v_stride_h, int32_t num_pages, int32_t page_size,
+                                    int64_t kc_stride_page, int64_t kc_stride_head, int64_t kc_stride_token,
+                                    int64_t vc_stride_page, int64_t vc_stride_head, int64_t vc_stride_token,
+                                    neso_stream_t stream);
+
+/* Attention of one query token per sequence, q [B, Hq, D], over the cached
+ * tokens t < seq_lens[b] (the new one included); query head h reads kv head
+ * h / (Hq / Hkv). D in {64, 128}.
+ *   s = scale q.k;  s = softcap tanh(s / softcap) if softcap > 0;
+ *   s += slopes[h] (t - (len - 1)) if slopes;  t > len - 1 - window if window > 0
+ *   out [B, Hq, D] = softmax(s) v, in q's type.
+ * With weights_in/weights_out (fp32 [B, Hkv, tokens], may be one buffer),
+ * weights_out[b, kv, t] = weights_in[b, kv, t] + the sum of the softmax
+ * weights of the kv head's query heads, for t < seq_lens[b]; the rest is left.
+ * A length is clamped to [0, table_width * page_size]; tokens of a page
+ * outside [0, num_pages) are left out; with no token left the row is zero. */
+NESO_API int neso_paged_attention(const void* q, const void* k_cache, const void* v_cache,
+                                  const int32_t* block_tables, const int32_t* seq_lens, const float* slopes,
+                                  const float* weights_in, float* weights_out, void* out, void* workspace,
+                                  int64_t workspace_bytes, int32_t dtype, int32_t B, int32_t Hq, int32_t Hkv,
+                                  int32_t D, float scale, float softcap, int32_t window, int64_t q_stride_b,
+                                  int64_t q_stride_h, int32_t num_pages, int32_t page_size, int64_t k_stride_page,
+                                  int64_t k_stride_head, int64_t k_stride_token, int64_t v_stride_page,
+                                  int64_t v_stride_head, int64_t v_stride_token, int32_t table_width,
+                                  int64_t table_stride, int64_t win_stride_b, int64_t win_stride_h,
+                                  int64_t wout_stride_b, int64_t wout_stride_h, neso_stream_t stream);
+/* Bytes of workspace that neso_paged_attention needs on the current device;
+ * negative (a status code) for arguments that it would refuse. */
+NESO_API int64_t neso_paged_attention_workspace(int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int32_t table_width,
+                                                int32_t page_size, int32_t with_weights);
+
+/* Trim every sequence to at most `budget` tokens per kv head: the first
+ * `sink`, the last `recent` and, of those between, the ones with the largest
+ * weight (ties: the lower index; NaN counts as largest) are kept, in order,
+ * and moved to tokens 0, 1, ... under out_tables. kept [B, Hkv, budget] gets
+ * their old indexes (-1 behind the last), new_lens[b] = min(len, budget)
+ * (a buffer other than seq_lens).
+ * weights_out [B, Hkv, tokens] gets the kept weights and zero up to the old
+ * length; it may be weights_in. out_tables may be block_tables (in place);
+ * otherwise its pages have to be other than every page of block_tables, and
+ * two sequences share none. Kept tokens past the out table's end, and tokens
+ * on a page outside [0, num_pages), are not moved. 16-bit elements; D a
+ * multiple of 8, at most 256. */
+NESO_API int neso_kv_evict(void* k_cache, void* v_cache, const int32_t* block_tables, const int32_t* out_tables,
+                           const int32_t* seq_lens, const float* weights_in, float* weights_out, int32_t* kept,
+                           int32_t* new_lens, int32_t B, int32_t Hkv, int32_t D, int32_t budget, int32_t recent,
+                           int32_t sink, int32_t num_pages, int32_t page_size, int64_t k_stride_page,
+                           int64_t k_stride_head, int64_t k_stride_token, int64_t v_stride_page,
+                           int64_t v_stride_head, int64_t v_stride_token, int32_t table_width, int64_t table_stride,
+                           int32_t out_width, int64_t out_stride, int64_t win_stride_b, int64_t win_stride_h,
+                           int64_t wout_stride_b, int64_t wout_stride_h, neso_stream_t stream);
+
+/* Logits of the next token, row by row (fp32 arithmetic, one rounding):
+ *   x = logits[b, v]
+ *   x = x > 0 ? x / repetition[b] : x * repetition[b]   if v is in the history
+ *   x -= frequency[b] * n + presence[b] * (n > 0)        n: times v was generated
+ *   x += bias[b, i] for each i with bias_ids[b, i] == v, in order
+ *   out[b, v] = -inf unless bit v % 32 of mask[b, v / 32] is set
+ * history [B, T] holds history_lens[b] token ids, the first prompt_lens[b] of
+ * them the prompt (counted for repetition only); ids outside [0, V) are
+ * skipped, lengths clamped to [0, T]. Any of history (with its lengths),
+ * prompt_lens (none: all generated), repetition, frequency, presence,
+ * bias_ids (with bias) and mask may be NULL. out may be logits itself. */
+NESO_API int neso_process_logits(const void* logits, void* out, int32_t dtype, int32_t B, int32_t V,
+                                 int64_t logits_stride, int64_t out_stride, const int32_t* history,
+                                 const int32_t* history_lens, const int32_t* prompt_lens, int32_t T,
+                                 int64_t history_stride, const float* repetition, const float* frequency,
+                                 const float* presence, const int32_t* bias_ids, const float* bias, int32_t num_bias,
+                                 const int32_t* mask, int64_t mask_stride, neso_stream_t stream);
 
 #ifdef __cplusplus
 }

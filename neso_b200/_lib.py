@@ -24,6 +24,11 @@ NESO_ERR_LAUNCH = -5
 NESO_ERR_DEVICE_TIMEOUT = -6
 NESO_ERR_NO_DEVICE = -7
 
+# Element types of the entry points that take more than one.
+NESO_F16 = 0
+NESO_BF16 = 1
+NESO_F32 = 2
+
 _CODE_NAMES = {
     NESO_OK: "NESO_OK",
     NESO_ERR_INVALID_ARG: "NESO_ERR_INVALID_ARG",
@@ -56,6 +61,7 @@ _u32 = ctypes.c_uint32
 _f32 = ctypes.c_float
 _int = ctypes.c_int
 _ip = ctypes.POINTER(ctypes.c_int)
+_i64 = ctypes.c_int64
 _GRID = [_u32, _u32, _u32]
 
 # name -> (restype, argtypes); kept in the order of include/neso_b200.h
@@ -94,6 +100,13 @@ SIGNATURES: dict[str, tuple[object, list]] = {
     "neso_w8a16_matmul_mnk": (_int, [_p, _p, _p, _p, _i32, _i32, _i32, _p]),
     "neso_w4a16_g128_matmul": (_int, [_p, _p, _p, _p, _i32, _i32, _i32, _p]),
     "neso_w8a16_matmul_mnk_noalloc": (_int, [_p, _p, _p, _p, _i32, _i32, _i32, _p]),
+    "neso_rope_paged_append": (_int, [_p] * 10 + [_i32] * 8 + [_p] + [_i64] * 6 + [_i32] * 2 + [_i64] * 6 + [_p]),
+    "neso_paged_attention": (_int, [_p] * 10 + [_i64] + [_i32] * 5 + [_f32] * 2 + [_i32] + [_i64] * 2 + [_i32] * 2
+                             + [_i64] * 6 + [_i32] + [_i64] * 5 + [_p]),
+    "neso_paged_attention_workspace": (_i64, [_i32] * 7),
+    "neso_kv_evict": (_int, [_p] * 9 + [_i32] * 8 + [_i64] * 6 + [_i32, _i64, _i32, _i64] + [_i64] * 4 + [_p]),
+    "neso_process_logits": (_int, [_p, _p, _i32, _i32, _i32, _i64, _i64, _p, _p, _p, _i32, _i64, _p, _p, _p, _p, _p,
+                                   _i32, _p, _i64, _p]),
 }
 
 _lib: ctypes.CDLL | None = None

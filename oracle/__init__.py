@@ -6,3 +6,4 @@ checker or the timed CPU baseline. The product path (``neso_b200``) never
 imports it and has no CPU fallback.
 """
 from .oracle import *  # noqa: F401,F403
+from .decode import *  # noqa: F401,F403

@@ -1,0 +1,727 @@
+"""One decoding step over a paged cache, on the GPU, against 64-bit definitions.
+
+Tolerances, in the order in which the terms arise (u = 2^-24, one fp32 rounding):
+
+* A score is a sum of D products that are exact in fp32, rounded at most D
+  times (twice u each where the tensor core truncates), then scaled, capped and
+  biased with a handful of roundings. With A = max_t sum_d |scale q_d k_d| and S
+  the largest score or bias, it is off by at most delta = 2u (D A + 8 S).
+* exp of it is off by the factor e^delta, the exponential's own 2^-21 and the
+  weight's 2^-16 (a 16-bit value and its 16-bit remainder, bf16 the coarser),
+  numerator and denominator both: at most 2 delta + 2^-14 of sum p |v|.
+* The result is rounded once to 16 bits: eps / 2 of it, 2^-25 where fp16 is subnormal.
+
+Rotations round three times in fp32 and once to 16 bits; logits four times in
+fp32 and once to their type; an eviction moves values and is exact.
+"""
+import math
+
+import pytest
+import torch
+
+import oracle
+from neso_b200 import _lib, ops
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+TYPES = [torch.float16, torch.bfloat16]
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _make_cache(g, dtype, pages, hkv, page, D, layout="hnd"):
+    """K and V with NaN everywhere; tests fill the visible tokens. Returns device tensors."""
+    if layout == "hnd":
+        k, v = (torch.full((pages, hkv, page, D), math.nan, dtype=dtype) for _ in range(2))
+        return k.cuda(), v.cuda()
+    if layout == "nhd":
+        k, v = (torch.full((pages, page, hkv, D), math.nan, dtype=dtype).cuda().transpose(1, 2) for _ in range(2))
+        return k, v
+    both = torch.full((pages, 2, hkv, page, D + 8), math.nan, dtype=dtype).cuda()  # joint buffer, padded rows
+    return both[:, 0, :, :, :D], both[:, 1, :, :, :D]
+
+
+def _fill(g, cache, table, n, scale=1.0):
+    """Random values for tokens 0..n-1 of one sequence."""
+    page, hkv, D = cache.shape[2], cache.shape[1], cache.shape[3]
+    x = (torch.randn(n, hkv, D, generator=g) * scale).to(cache.dtype).cuda()
+    for t in range(0, n, page):
+        m = min(page, n - t)
+        cache[int(table[t // page]), :, :m] = x[t:t + m].transpose(0, 1)
+
+
+def _setup(seed, dtype, lens, hq, hkv, D, page, layout="hnd", extra_width=0, spare=3):
+    g = _gen(seed)
+    need = [-(-max(n, 0) // page) for n in lens]
+    width = max(need + [0]) + extra_width
+    pages = sum(need) + spare
+    order = torch.randperm(pages, generator=g)[:sum(need)].tolist()
+    table = torch.full((len(lens), width), -1, dtype=torch.int32)
+    for b, m in enumerate(need):
+        table[b, :m] = torch.tensor([order.pop() for _ in range(m)], dtype=torch.int32)
+    k, v = _make_cache(g, dtype, pages, hkv, page, D, layout)
+    for b, n in enumerate(lens):
+        _fill(g, k, table[b], max(n, 0))
+        _fill(g, v, table[b], max(n, 0))
+    q = (torch.randn(len(lens), hq, D, generator=g) * 1.5).to(dtype).cuda()
+    return q, k, v, table, torch.tensor(lens, dtype=torch.int32), g
+
+
+def _attention_tolerance(out, bounds, dtype, D, biggest):
+    delta = 2 * U * (D * bounds[..., :1] + 8 * biggest)
+    return (2 * delta + 2.0 ** -14) * bounds[..., 1:] + torch.finfo(dtype).eps / 2 * out.abs() + 2.0 ** -25
+
+
+def _check_attention(q, k, v, table, lens, D, dtype, scale=None, softcap=0.0, window=0, slopes=None, weights=None,
+                     **kw):
+    s = 1 / math.sqrt(D) if scale is None else scale
+    got = ops.paged_attention(q, k, v, table.cuda(), lens.cuda(), scale=scale, softcap=softcap, window=window,
+                              slopes=None if slopes is None else slopes.cuda(), weights=weights, **kw)
+    ref, sums, bounds = oracle.decode_attention(q.cpu(), k.cpu(), v.cpu(), table, lens, s, softcap, window, slopes)
+    span = window if window else int(max(lens.max(), 0))
+    biggest = float(bounds[..., 0].max()) + (float(slopes.abs().max()) * span if slopes is not None else 0.0)
+    tol = _attention_tolerance(ref, bounds, dtype, D, biggest)
+    err = (got.cpu().double() - ref).abs()
+    assert got.dtype == dtype and bool((err <= tol).all()), float((err - tol).max())
+    return got, sums, 2 * 2 * U * (D * float(bounds[..., 0].max()) + 8 * biggest) + 2.0 ** -19
+
+
+# ------------------------------------------------------------ attention ----
+ATTENTION = [
+    # lens, hq, hkv, D, page
+    ([1], 1, 1, 64, 16),
+    ([1], 8, 1, 128, 16),
+    ([0, 1, 2, 15, 16, 17, 33], 4, 2, 64, 16),
+    ([129], 16, 16, 64, 16),
+    ([700, 5, 0, 64, 1], 8, 1, 128, 7),
+    ([40, 250], 9, 1, 64, 1),          # pages of one token, group of nine
+    ([257, 31], 32, 2, 128, 24),       # group of sixteen, pages that end inside a unit
+    ([100, 3], 20, 1, 64, 256),        # group of twenty: two passes of ten
+    ([65, 300], 50, 1, 128, 32),       # group of fifty: four passes, the last short
+    ([1000, 999, 998], 6, 2, 128, 128),
+    ([0, 0], 4, 4, 64, 16),
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("case", range(len(ATTENTION)))
+def test_attention_shapes(dev, case, dtype):
+    lens, hq, hkv, D, page = ATTENTION[case]
+    q, k, v, table, n, _ = _setup(case, dtype, lens, hq, hkv, D, page)
+    _check_attention(q, k, v, table, n, D, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("window", [1, 15, 16, 17, 100])
+def test_attention_window(dev, window, dtype):
+    q, k, v, table, n, _ = _setup(window, dtype, [1, 16, 99, 100, 101, 333], 8, 2, 64, 24)
+    # what the window hides may be anything
+    for b, length in enumerate(n.tolist()):
+        for t in range(max(0, length - window)):
+            k[int(table[b, t // 24]), :, t % 24] = math.inf
+            v[int(table[b, t // 24]), :, t % 24] = math.nan
+    _check_attention(q, k, v, table, n, 64, dtype, window=window)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("softcap,use_slopes,window", [(5.0, False, 0), (0.0, True, 0), (30.0, True, 50)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_attention_bias(dev, D, softcap, use_slopes, window, dtype):
+    q, k, v, table, n, g = _setup(7, dtype, [200, 33, 1, 0], 12, 2, D, 16)
+    slopes = torch.rand(12, generator=g) * 0.3 - 0.05 if use_slopes else None
+    _check_attention(q, k, v, table, n, D, dtype, softcap=softcap, slopes=slopes, window=window)
+
+
+@pytest.mark.parametrize("layout", ["nhd", "joint"])
+def test_attention_strides(dev, layout):
+    q, k, v, table, n, _ = _setup(11, torch.float16, [130, 17], 8, 4, 64, 16, layout=layout)
+    wide = torch.full((2, 12, 72), math.nan, dtype=torch.float16, device=dev)  # q inside a fused projection
+    wide[:, 2:10, :64] = q
+    _check_attention(wide[:, 2:10, :64], k, v, table, n, 64, torch.float16)
+    tw = torch.full((2, table.shape[1] + 5), 0, dtype=torch.int32, device=dev)
+    tw[:, :table.shape[1]] = table.to(dev)
+    a = ops.paged_attention(q, k, v, tw[:, :table.shape[1]], n.cuda())
+    assert torch.equal(a, ops.paged_attention(q, k, v, table.cuda(), n.cuda()))
+
+
+def test_attention_extreme_scores(dev):
+    # one token far above the rest; scores of +-30000 at scale 1; -inf keys leave their token out
+    q, k, v, table, n, _ = _setup(12, torch.float16, [90], 2, 2, 64, 16)
+    q[:] = 0
+    q[:, :, 0] = 60.0
+    k[:, :, :, 0] = torch.where(k[:, :, :, 0].isnan(), k[:, :, :, 0], torch.full_like(k[:, :, :, 0], -500.0))
+    t = 77
+    k[int(table[0, t // 16]), :, t % 16, 0] = 500.0
+    got = ops.paged_attention(q, k, v, table.cuda(), n.cuda(), scale=1.0)
+    assert torch.equal(got[0], v[int(table[0, t // 16]), :, t % 16])
+    k[int(table[0, 0]), :, 3, 0] = -math.inf
+    assert torch.equal(got, ops.paged_attention(q, k, v, table.cuda(), n.cuda(), scale=1.0))
+    # a NaN key that is visible shows
+    k[int(table[0, 0]), 0, 3, 1] = math.nan
+    got = ops.paged_attention(q, k, v, table.cuda(), n.cuda(), scale=1.0)
+    assert bool(got[0, 0].isnan().all()) and not bool(got[0, 1].isnan().any())
+
+
+def test_attention_bad_pages_and_lengths(dev):
+    # pages outside the cache are left out, lengths are clamped to the table
+    q, k, v, table, n, _ = _setup(13, torch.float16, [100, 64, 50, 40], 4, 2, 64, 16)
+    table[0, 1], table[0, 5] = -7, 10 ** 6
+    table[1, :] = -1
+    n = torch.tensor([100, 64, -5, 2 ** 31 - 1], dtype=torch.int32)
+    table[3, :] = table[3, 0]  # every page the same, so that all of the table is valid
+    k[int(table[3, 0])] = 0.5
+    v[int(table[3, 0])] = torch.randn(v.shape[1:], generator=_gen(1)).half().cuda()
+    got, _, _ = _check_attention(q, k, v, table, n, 64, torch.float16)
+    assert bool((got[1] == 0).all()) and bool((got[2] == 0).all())
+    # no pages, no table: zeros
+    empty = torch.empty(0, 2, 16, 64, dtype=torch.float16, device=dev)
+    assert bool((ops.paged_attention(q, empty, empty, table.cuda(), n.cuda()) == 0).all())
+    assert bool((ops.paged_attention(q, k, v, table[:, :0].cuda(), n.cuda()) == 0).all())
+    assert ops.paged_attention(q[:0], k, v, table[:0].cuda(), n[:0].cuda()).shape == (0, 4, 64)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hq,hkv,D,window", [(4, 4, 64, 0), (8, 1, 128, 0), (20, 1, 64, 0), (6, 2, 128, 40)])
+def test_attention_weights(dev, hq, hkv, D, window, dtype):
+    lens = [0, 1, 31, 150, 700]
+    q, k, v, table, n, g = _setup(hq, dtype, lens, hq, hkv, D, 16, extra_width=2)
+    tokens = table.shape[1] * 16 + 3
+    before = torch.rand(5, hkv, tokens, generator=g)
+    after = torch.full_like(before, -1.0).cuda()
+    given = before.cuda()
+    got, sums, tol = _check_attention(q, k, v, table, n, D, dtype, window=window, weights=given, weights_out=after)
+    assert torch.equal(given.cpu(), before)
+    plain = ops.paged_attention(q, k, v, table.cuda(), n.cuda(), window=window)
+    assert torch.equal(plain, got)
+    for b, length in enumerate(lens):
+        for kv in range(hkv):
+            add = torch.zeros(tokens, dtype=torch.float64)
+            for t, x in sums.get((b, kv), {}).items():
+                add[t] = x
+            want = before[b, kv].double() + add
+            bound = tol * add + 2 * U * want + 2.0 ** -60
+            assert bool(((after[b, kv].cpu().double() - want).abs() <= bound)[:length].all())
+            assert bool((after[b, kv, length:] == -1.0).all())
+    ops.paged_attention(q, k, v, table.cuda(), n.cuda(), window=window, weights=given)
+    for b, length in enumerate(lens):
+        assert torch.equal(given[b, :, :length], after[b, :, :length])
+        assert torch.equal(given[b, :, length:].cpu(), before[b, :, length:])
+
+
+def test_attention_long_and_far(dev):
+    # a cache of more than 2^32 elements, the sequences' pages at both ends; many runs per head are joined
+    D, hkv, page, lens = 128, 8, 64, [20011, 37]
+    pages = (1 << 32) // (2 * hkv * page * D) + 400
+    both = torch.empty(pages, 2, hkv, page, D, dtype=torch.float16, device=dev)
+    k, v = both[:, 0], both[:, 1]
+    width = -(-lens[0] // page)
+    table = torch.zeros(2, width, dtype=torch.int32)
+    table[0] = torch.arange(pages - width, pages, dtype=torch.int32).flip(0)
+    table[0, ::2] = torch.arange(0, width, dtype=torch.int32)[::2]
+    table[1, 0] = pages - width - 1
+    g = torch.Generator(device=dev).manual_seed(5)
+    for b in range(2):
+        rows = table[b, :-(-lens[b] // page)].long().to(dev)
+        for c in (k, v):
+            c[rows] = torch.randn(len(rows), hkv, page, D, device=dev, generator=g).half()
+    q = torch.randn(2, 32, D, device=dev, generator=g).half()
+    got = ops.paged_attention(q, k, v, table.to(dev), torch.tensor(lens, dtype=torch.int32, device=dev))
+    for b in range(2):
+        rows = table[b, :-(-lens[b] // page)].long().to(dev)
+        kk, vv = (c[rows].transpose(0, 1).flatten(1, 2)[:, :lens[b]].double() for c in (k, v))
+        qq = q[b].double().view(hkv, 4, D) / math.sqrt(D)
+        p = torch.softmax(qq @ kk.transpose(1, 2), -1)
+        ref = (p @ vv).view(32, D)
+        big = float((qq.abs() @ kk.abs().transpose(1, 2)).max())
+        bounds = torch.stack([torch.full((32,), big, dtype=torch.float64, device=dev),
+                              (p @ vv.abs()).view(32, D).amax(-1)], -1)
+        tol = _attention_tolerance(ref, bounds, torch.float16, D, big)
+        assert bool(((got[b].double() - ref).abs() <= tol).all())
+
+
+def test_attention_repeats_and_streams(dev):
+    q, k, v, table, n, _ = _setup(21, torch.bfloat16, [500, 3, 900, 77] * 8, 16, 4, 128, 16)
+    table, n = table.cuda(), n.cuda()
+    first = ops.paged_attention(q, k, v, table, n)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    outs = []
+    for _ in range(4):
+        for s in streams:  # calls that overlap on the GPU have workspaces of their own
+            with torch.cuda.stream(s):
+                outs.append(ops.paged_attention(q, k, v, table, n))
+    torch.cuda.synchronize()
+    assert all(torch.equal(first, o) for o in outs)
+
+
+def test_attention_graphs_follow_lengths(dev):
+    q, k, v, table, n, _ = _setup(22, torch.float16, [300, 40], 8, 2, 64, 16)
+    table, n = table.cuda(), n.cuda()
+    w = torch.zeros(2, 2, table.shape[1] * 16, device=dev)
+    ops.paged_attention(q, k, v, table, n)  # loads the kernels before the capture
+    ops.paged_attention(q, k, v, table, n, weights=w.clone())
+    graphs, outs = [], []
+    pool_stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=pool_stream):
+            outs.append(ops.paged_attention(q, k, v, table, n, weights=w))
+        graphs.append(g)
+    for lens in ([300, 40], [17, 0], [299, 1]):
+        n.copy_(torch.tensor(lens, dtype=torch.int32))
+        want_w = w.clone()
+        want = ops.paged_attention(q, k, v, table, n, weights=want_w)
+        ops.paged_attention(q, k, v, table, n, weights=want_w)
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want) and torch.equal(outs[1], want) and torch.equal(w, want_w)
+
+
+def test_attention_refusals(dev):
+    q, k, v, table, n, _ = _setup(23, torch.float16, [20, 3], 4, 2, 64, 16)
+    table, n = table.cuda(), n.cuda()
+    call = ops.paged_attention
+    with pytest.raises(TypeError):
+        call(q.float(), k, v, table, n)
+    with pytest.raises(TypeError):
+        call(q, k, v, table.long(), n)
+    with pytest.raises(TypeError):
+        call(q, k, v.bfloat16(), table, n)
+    with pytest.raises(ValueError):
+        call(q.cpu(), k, v, table, n)
+    with pytest.raises(ValueError):
+        call(q, k, v, table, n.cpu())
+    with pytest.raises(ValueError):
+        call(q, k, v, table, n[:1])
+    with pytest.raises(ValueError):
+        call(q, k.transpose(2, 3), v.transpose(2, 3), table, n)
+    with pytest.raises(ValueError):
+        call(q, k, v, table, n, out=q)
+    with pytest.raises(ValueError):
+        call(q, k, v, table, n, weights=torch.zeros(2, 2, 31, device=dev))
+    w = torch.zeros(2, 2, 100, device=dev)
+    with pytest.raises(ValueError):
+        call(q, k, v, table, n, weights=w[:, :, :64], weights_out=w[:, :, 1:65])
+    with pytest.raises(_lib.NesoError, match="UNSUPPORTED"):
+        call(q[..., :32].contiguous(), k[..., :32].contiguous(), v[..., :32].contiguous(), table, n)
+    with pytest.raises(_lib.NesoError, match="multiple"):
+        call(q[:, :3].contiguous(), k, v, table, n)
+    with pytest.raises(_lib.NesoError, match="softcap"):
+        call(q, k, v, table, n, softcap=-1.0)
+    with pytest.raises(_lib.NesoError, match="window"):
+        call(q, k, v, table, n, window=-1)
+    odd = torch.zeros(k.numel() + 1, dtype=torch.float16, device=dev)[1:].view(k.shape)
+    with pytest.raises(_lib.NesoError, match="MISALIGNED"):
+        call(q, odd, v, table, n)
+
+
+# --------------------------------------------------------------- append ----
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N,hq,hkv,D,half,sections,page", [
+    (1, 4, 2, 64, 32, None, 16),
+    (7, 3, 1, 128, 64, [20, 22, 22], 5),
+    (33, 2, 2, 64, 12, [12, 0], 16),       # a rotated part that is no multiple of eight
+    (5, 1, 1, 80, 24, None, 1),
+    (2, 1, 1, 64, 0, None, 16),            # nothing is rotated
+    (300, 8, 8, 64, 32, None, 16),
+])
+def test_append(dev, N, hq, hkv, D, half, sections, page, dtype):
+    g = _gen(N + D)
+    q, k, v = ((torch.randn(N, h, D, generator=g) * 3).to(dtype) for h in (hq, hkv, hkv))
+    axes = len(sections) if sections else 1
+    angle = torch.rand(50, half, generator=g) * 6.28
+    cos, sin = angle.cos(), angle.sin()
+    pos = torch.randint(0, 50, (axes, N), generator=g, dtype=torch.int32)
+    pages = -(-N // page) + 2
+    slots = torch.randperm(pages * page, generator=g)[:N]
+    if N > 4:
+        slots[2], slots[3] = -1, pages * page  # padding
+        pos[0, 4] = 50                         # outside the table
+    for fused in (False, True):
+        if fused:
+            buf = torch.cat([q, k, v], 1).cuda()
+            qd, kd, vd = buf[:, :hq], buf[:, hq:hq + hkv], buf[:, hq + hkv:]
+        else:
+            qd, kd, vd = q.cuda(), k.cuda(), v.cuda()
+        kc, vc = (torch.full((pages, hkv, page, D), 7.0, dtype=dtype, device=dev) for _ in range(2))
+        got = ops.rope_paged_append(qd, kd, vd, cos.cuda(), sin.cuda(), pos.cuda() if axes > 1 else pos[0].cuda(),
+                                    slots.cuda(), kc, vc, sections=sections)
+        refs = [oracle.decode_rope(x, cos, sin, pos, sections or [half]) for x in (q, k)]
+        mags = [oracle.decode_rope(x.abs(), cos.abs(), -sin.abs(), pos, sections or [half]).abs() for x in (q, k)]
+        want_k, want_v = (torch.full((pages, hkv, page, D), 7.0, dtype=torch.float64) for _ in range(2))
+        tol_k = torch.zeros_like(want_k)
+        eps = torch.finfo(dtype).eps / 2
+        for i in range(N):
+            s = int(slots[i])
+            if 0 <= s < pages * page:
+                want_k[s // page, :, s % page] = refs[1][i]
+                # |u c| + |w s| bounds both rotated elements of a pair
+                tol_k[s // page, :, s % page] = eps * refs[1][i].abs() + 6 * U * _pair_bound(mags[1][i], half) + 2.0 ** -25
+                want_v[s // page, :, s % page] = v[i].double()
+            else:
+                refs[0][i] = 0
+        tol_q = eps * refs[0].abs() + 6 * U * _pair_bound(mags[0], half) + 2.0 ** -25
+        _close(got, refs[0], tol_q)
+        _close(kc, want_k, tol_k)
+        _close(vc, want_v, torch.zeros_like(want_v))
+
+
+def _pair_bound(m, half):
+    """The larger magnitude of each rotated pair, for both of its elements."""
+    m = m.clone()
+    top = torch.maximum(m[..., :half], m[..., half:2 * half])
+    m[..., :half] = top
+    m[..., half:2 * half] = top
+    return m
+
+
+def _close(got, want, tol):
+    got = got.cpu().double()
+    same_nan = torch.equal(got.isnan(), want.isnan())
+    err = (got - want).abs()
+    assert same_nan and bool((err <= tol)[~want.isnan()].all())
+
+
+def test_append_in_place_streams_and_graph(dev):
+    g = torch.Generator(device=dev).manual_seed(3)
+    q, k, v = (torch.randn(40, h, 64, device=dev, generator=g).half() for h in (4, 2, 2))
+    cos, sin = torch.rand(64, 32, device=dev, generator=g), torch.rand(64, 32, device=dev, generator=g)
+    pos = torch.arange(40, dtype=torch.int32, device=dev)
+    slots = torch.arange(40, device=dev)
+    kc, vc = (torch.zeros(4, 2, 16, 64, dtype=torch.float16, device=dev) for _ in range(2))
+    want = ops.rope_paged_append(q, k, v, cos, sin, pos, slots, kc, vc)
+    k1, v1 = kc.clone(), vc.clone()
+    x = q.clone()
+    assert ops.rope_paged_append(x, k, v, cos, sin, pos, slots, kc, vc, out=x) is x and torch.equal(x, want)
+    out = torch.empty_like(q)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.rope_paged_append(q, k, v, cos, sin, pos, slots, kc, vc, out=out)
+    kc.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and torch.equal(kc, k1) and torch.equal(vc, v1)
+    # strided rows that are not on 16 bytes take the scalar form: same values
+    wide = torch.empty(40, 8, 65, dtype=torch.float16, device=dev)
+    wide[:, :4, 1:], wide[:, 4:6, 1:], wide[:, 6:, 1:] = q, k, v
+    kc.zero_()
+    got = ops.rope_paged_append(wide[:, :4, 1:], wide[:, 4:6, 1:], wide[:, 6:, 1:], cos, sin, pos, slots, kc, vc)
+    assert torch.equal(got, want) and torch.equal(kc, k1)
+
+
+def test_append_refusals(dev):
+    q, k = torch.zeros(3, 4, 64, dtype=torch.float16, device=dev), torch.zeros(3, 2, 64, dtype=torch.float16, device=dev)
+    cos = torch.zeros(10, 32, device=dev)
+    pos, slots = torch.zeros(3, dtype=torch.int32, device=dev), torch.arange(3, device=dev)
+    kc = torch.zeros(2, 2, 16, 64, dtype=torch.float16, device=dev)
+    vc = kc.clone()
+    call = ops.rope_paged_append
+    with pytest.raises(TypeError):
+        call(q, k, k, cos.double(), cos.double(), pos, slots, kc, vc)
+    with pytest.raises(TypeError):
+        call(q, k, k, cos, cos, pos, slots.int(), kc, vc)
+    with pytest.raises(ValueError):
+        call(q, k[:2], k, cos, cos, pos, slots, kc, vc)
+    with pytest.raises(ValueError):
+        call(q, k, k, cos, cos, torch.zeros(2, 3, dtype=torch.int32, device=dev), slots, kc, vc)
+    with pytest.raises(ValueError):
+        call(q, k, k, cos, cos, pos, slots, kc[:1].expand(2, 2, 16, 64), vc)
+    big = torch.zeros(4, 4, 64, dtype=torch.float16, device=dev)
+    with pytest.raises(ValueError, match="overlap"):
+        call(big[:3], k, k, cos, cos, pos, slots, kc, vc, out=big[1:])
+    with pytest.raises(_lib.NesoError, match="sections"):
+        call(q, k, k, cos, cos, torch.zeros(2, 3, dtype=torch.int32, device=dev), slots, kc, vc, sections=[16, 15])
+    wide = torch.zeros(10, 40, device=dev)
+    with pytest.raises(_lib.NesoError, match="rotates more"):
+        call(q, k, k, wide, wide, pos, slots, kc, vc)
+
+
+# ---------------------------------------------------------------- evict ----
+def _check_evict(seed, dtype, lens, hkv, D, page, budget, recent, sink, mode, weights=None, layout="hnd", extra=0):
+    q, k, v, table, n, g = _setup(seed, dtype, lens, hkv, hkv, D, page, layout=layout, extra_width=extra,
+                                  spare=3 + len(lens) * (-(-budget // page)))
+    tokens = table.shape[1] * page
+    if weights is None:
+        weights = torch.rand(len(lens), hkv, tokens, generator=g)
+        weights = torch.where(weights < 0.2, torch.zeros(()), weights).mul(8).round().div(8)  # many ties
+    before = weights.clone()
+    kept_ref = oracle.decode_evict(before, n, budget, recent, sink, tokens)
+    out_table = table
+    if mode == "apart":
+        free = sorted(set(range(k.shape[0])) - set(table[table >= 0].tolist()))
+        width = -(-budget // page)
+        out_table = torch.tensor(free[:len(lens) * width], dtype=torch.int32).view(len(lens), width)
+    k0, v0 = k.cpu().clone(), v.cpu().clone()
+    w = weights.cuda()
+    w_out = torch.full_like(w, -3.0) if mode == "apart" else None
+    kept, new = ops.kv_evict(k, v, table.cuda(), n.cuda(), w, budget, recent, sink=sink,
+                             out_tables=out_table.cuda() if mode == "apart" else None, weights_out=w_out)
+    after = w if w_out is None else w_out
+    want_k, want_v = k0.clone(), v0.clone()
+    want_w = before.clone() if w_out is None else torch.full_like(before, -3.0)
+    for b, length in enumerate(lens):
+        assert int(new[b]) == min(length, budget)
+        for h in range(hkv):
+            rows = kept_ref[b][h]
+            assert kept[b, h].tolist() == rows + [-1] * (budget - len(rows))
+            for j, t in enumerate(rows):
+                src, dst = (int(table[b, t // page]), t % page), (int(out_table[b, j // page]), j % page)
+                want_k[dst[0], h, dst[1]] = k0[src[0], h, src[1]]
+                want_v[dst[0], h, dst[1]] = v0[src[0], h, src[1]]
+            want_w[b, h, :len(rows)] = before[b, h, rows]
+            want_w[b, h, len(rows):length] = 0
+    torch.testing.assert_close(k.cpu(), want_k, rtol=0, atol=0, equal_nan=True)
+    torch.testing.assert_close(v.cpu(), want_v, rtol=0, atol=0, equal_nan=True)
+    torch.testing.assert_close(after.cpu(), want_w, rtol=0, atol=0, equal_nan=True)
+
+
+@pytest.mark.parametrize("mode", ["in_place", "apart"])
+@pytest.mark.parametrize("lens,hkv,D,page,budget,recent,sink", [
+    ([1], 1, 64, 16, 1, 0, 0),
+    ([0, 1, 5, 17], 2, 64, 4, 5, 2, 1),
+    ([100, 37, 64], 2, 128, 16, 32, 0, 0),
+    ([100, 37, 64], 1, 128, 7, 32, 32, 0),     # nothing but the recent ones
+    ([100, 37, 64], 1, 64, 7, 32, 10, 22),     # nothing is chosen
+    ([333, 9], 3, 8, 24, 300, 100, 4),
+    ([50], 1, 256, 16, 49, 0, 49),
+    ([5000], 2, 64, 64, 4321, 17, 3),
+])
+def test_evict(dev, lens, hkv, D, page, budget, recent, sink, mode):
+    _check_evict(len(lens) + D, TYPES[D % 3 % 2], lens, hkv, D, page, budget, recent, sink, mode)
+
+
+@pytest.mark.parametrize("mode", ["in_place", "apart"])
+def test_evict_special_weights(dev, mode):
+    w = torch.zeros(2, 1, 64)
+    w[0, 0] = torch.arange(64.0).flip(0) - 32.0
+    w[0, 0, [5, 40]] = math.nan
+    w[0, 0, [3, 60]] = math.inf
+    w[0, 0, 7] = -math.inf
+    w[1, 0, ::2] = -0.0  # ties with +0
+    _check_evict(1, torch.float16, [64, 61], 1, 64, 16, 20, 3, 2, mode, weights=w)
+
+
+def test_evict_strided_cache_and_spare_table(dev):
+    _check_evict(2, torch.float16, [90, 20], 2, 64, 16, 30, 8, 2, "in_place", layout="nhd", extra=4)
+    _check_evict(3, torch.float16, [90, 20], 2, 64, 16, 30, 8, 2, "apart", layout="joint", extra=4)
+
+
+def test_evict_bad_pages_and_lengths(dev):
+    # rows on a page outside the cache are not moved; nothing else is touched
+    q, k, v, table, n, g = _setup(4, torch.float16, [64], 1, 1, 64, 16)
+    table[0, 2] = -1
+    w = torch.zeros(1, 1, 64)
+    w[0, 0, 40:44] = 1.0
+    k0 = k.clone()
+    kept, new = ops.kv_evict(k, v, table.cuda(), n.cuda(), w.cuda(), 10, 4)
+    assert kept[0, 0].tolist() == [0, 1, 40, 41, 42, 43, 60, 61, 62, 63] and int(new[0]) == 10
+    want = k0.clone()
+    for j, t in enumerate(kept[0, 0].tolist()):
+        if t // 16 != 2:
+            want[int(table[0, 0]), 0, j] = k0[int(table[0, t // 16]), 0, t % 16]
+    torch.testing.assert_close(k, want, rtol=0, atol=0, equal_nan=True)
+    big = torch.tensor([2 ** 31 - 1], dtype=torch.int32, device=dev)
+    table[0, 2] = 0
+    _, new = ops.kv_evict(k, v, table.cuda(), big, w.cuda(), 64, 4)
+    assert int(new[0]) == 64
+    assert ops.kv_evict(k, v, table[:0].cuda(), n[:0].cuda(), w[:0].cuda(), 4, 0)[0].shape == (0, 1, 4)
+
+
+def test_evict_refusals(dev):
+    q, k, v, table, n, _ = _setup(5, torch.float16, [30], 2, 2, 64, 16)
+    w = torch.zeros(1, 2, 32, device=dev)
+    table, n = table.cuda(), n.cuda()
+    for budget, recent, sink in ((0, 0, 0), (4, 5, 0), (4, 2, 3), (4, -1, 0)):
+        with pytest.raises((_lib.NesoError, ValueError)):
+            ops.kv_evict(k, v, table, n, w, budget, recent, sink=sink)
+    with pytest.raises(ValueError):
+        ops.kv_evict(k, v, table, n, w[:, :, :31], 8, 2)
+    with pytest.raises(ValueError, match="out_tables"):
+        ops.kv_evict(k, v, table, n, w, 20, 2, out_tables=table[:, :1])
+    with pytest.raises(TypeError):
+        ops.kv_evict(k, v, table, n, w.double(), 8, 2)
+    wide = torch.zeros(1, 2, 40, device=dev)
+    with pytest.raises(ValueError, match="overlap"):
+        ops.kv_evict(k, v, table, n, wide[:, :, :32], 8, 2, weights_out=wide[:, :, 4:36])
+
+
+# --------------------------------------------------------------- logits ----
+def _logit_inputs(seed, B, V, T, dtype, n_bias=5):
+    g = _gen(seed)
+    x = (torch.randn(B, V, generator=g) * 5).to(dtype)
+    hist = torch.randint(0, max(1, min(V, 40)), (B, T), generator=g, dtype=torch.int32)
+    hist[:, ::5] = torch.randint(0, V, hist[:, ::5].shape, generator=g, dtype=torch.int32)
+    lens = torch.randint(0, T + 1, (B,), generator=g, dtype=torch.int32)
+    lens[0] = T
+    prompt = torch.randint(0, T + 1, (B,), generator=g, dtype=torch.int32)
+    rep, freq, pres = 1 + torch.rand(B, generator=g), torch.rand(B, generator=g) - 0.3, torch.rand(B, generator=g)
+    ids = torch.randint(0, V, (B, n_bias), generator=g, dtype=torch.int32)
+    bias = torch.randn(B, n_bias, generator=g) * 3
+    words = -(-V // 32)
+    mask = torch.randint(-(1 << 31), 1 << 31, (B, words), generator=g).to(torch.int32)
+    return x, dict(history=hist, history_lens=lens, prompt_lens=prompt, repetition=rep, frequency=freq, presence=pres,
+                   bias_ids=ids, bias=bias, mask=mask)
+
+
+def _check_logits(x, kw, xd=None, out=None):
+    got = ops.process_logits(x.cuda() if xd is None else xd, out=out,
+                             **{k: None if v is None else v.cuda() for k, v in kw.items()})
+    want, mag = oracle.decode_logits(x, **kw)
+    eps = torch.finfo(x.dtype).eps / 2
+    n = kw["bias"].shape[1] if kw.get("bias") is not None else 0
+    tol = (5 + n) * U * mag + eps * want.abs() + (2.0 ** -25 if x.dtype == torch.float16 else 0)
+    g = got.cpu().double()
+    fin = want.isfinite()
+    torch.testing.assert_close(g[~fin], want[~fin], rtol=0, atol=0, equal_nan=True)
+    assert bool(((g - want).abs() <= tol)[fin].all())
+    return got
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("B,V,T", [(1, 1, 1), (3, 31, 7), (2, 33, 50), (2, 8187, 100), (3, 8193, 64), (1, 20001, 300)])
+def test_logits(dev, B, V, T, dtype):
+    x, kw = _logit_inputs(V, B, V, T, dtype)
+    kw["mask"][0] = 0 if B > 1 else -1  # a row whose mask leaves nothing
+    _check_logits(x, kw)
+
+
+@pytest.mark.parametrize("names", [(), ("mask",), ("bias_ids", "bias"), ("history", "history_lens", "repetition"),
+                                   ("history", "history_lens", "frequency"),
+                                   ("history", "history_lens", "prompt_lens", "presence")])
+def test_logits_parts(dev, names):
+    x, kw = _logit_inputs(5, 2, 700, 90, torch.float32)
+    _check_logits(x, {k: v for k, v in kw.items() if k in names})
+
+
+def test_logits_odd_indexes(dev):
+    # ids outside the vocabulary are skipped, lengths clamped, the same biased token adds up in order
+    x, kw = _logit_inputs(6, 3, 500, 40, torch.float32)
+    kw["history"][:, 3], kw["history"][:, 4], kw["history"][:, 5] = -1, 500, 2 ** 31 - 1
+    kw["history_lens"] = torch.tensor([-4, 1000, 40], dtype=torch.int32)
+    kw["prompt_lens"] = torch.tensor([0, -3, 1000], dtype=torch.int32)
+    kw["bias_ids"] = torch.tensor([[7, 7, -1, 7, 499]] * 3, dtype=torch.int32)
+    kw["mask"][:, 0] |= 128
+    _check_logits(x, kw)
+    x[0, 0], x[0, 1], x[0, 2] = math.inf, -math.inf, math.nan
+    kw["mask"] = torch.full((3, 16), -1, dtype=torch.int32)
+    got = _check_logits(x, kw)
+    assert bool(got[0, 2].isnan())
+    kw["mask"] = torch.zeros(3, 20, dtype=torch.int32)
+    assert bool((_check_logits(x, kw) == -math.inf).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_logits_strides_and_in_place(dev, dtype):
+    x, kw = _logit_inputs(8, 4, 9001, 30, dtype)
+    base = _check_logits(x, kw)
+    for shift in (1, 3):  # rows off the vector boundary, odd pitch
+        wide = torch.zeros(4, 9011, dtype=dtype, device=dev)
+        view = wide[:, shift:shift + 9001]
+        view.copy_(x)
+        assert torch.equal(_check_logits(x, kw, xd=view), base)
+        other = torch.zeros(4, 9011, dtype=dtype, device=dev)
+        assert torch.equal(_check_logits(x, kw, xd=view, out=other[:, shift:shift + 9001]), base)
+        assert bool((other[:, :shift] == 0).all()) and bool((other[:, shift + 9001:] == 0).all())
+        assert torch.equal(_check_logits(x, kw, xd=view, out=view), base)
+        assert bool((wide[:, :shift] == 0).all()) and bool((wide[:, shift + 9001:] == 0).all())
+
+
+def test_logits_graph(dev):
+    x, kw = _logit_inputs(9, 2, 4000, 50, torch.float32)
+    kw = {k: v.cuda() for k, v in kw.items()}
+    x = x.cuda()
+    want = ops.process_logits(x, **kw)
+    out = torch.empty_like(x)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ops.process_logits(x, out=out, **kw)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+    kw["history_lens"].fill_(3)
+    g.replay()
+    assert torch.equal(out, ops.process_logits(x, **kw))
+
+
+def test_logits_refusals(dev):
+    x = torch.zeros(2, 100, device=dev)
+    ids = torch.zeros(2, 3, dtype=torch.int32, device=dev)
+    with pytest.raises(TypeError):
+        ops.process_logits(x.double())
+    with pytest.raises(ValueError):
+        ops.process_logits(x, history=ids)
+    with pytest.raises(ValueError):
+        ops.process_logits(x, repetition=torch.ones(2, device=dev))
+    with pytest.raises(ValueError):
+        ops.process_logits(x, bias_ids=ids)
+    with pytest.raises(ValueError):
+        ops.process_logits(x, mask=torch.zeros(2, 3, dtype=torch.int32, device=dev))
+    with pytest.raises(ValueError):
+        ops.process_logits(x.t())
+    with pytest.raises(ValueError, match="overlap"):
+        big = torch.zeros(2, 128, device=dev)
+        ops.process_logits(big[:, :100], out=big[:, 1:101])
+
+
+# ------------------------------------------------------------- together ----
+def test_decoding_steps_together(dev):
+    """Prompt, a few decoding steps, an eviction, more steps: the cache, the
+    accumulated weights and the outputs follow the 64-bit definitions."""
+    D, hq, hkv, page, B, V = 64, 4, 2, 16, 2, 300
+    g = _gen(99)
+    lens = [37, 20]
+    tables = torch.arange(8, dtype=torch.int32).view(2, 4).flip(0).contiguous()
+    kc, vc = (torch.zeros(8, hkv, page, D, dtype=torch.float16, device=dev) for _ in range(2))
+    angle = torch.rand(200, 32, generator=g) * 6.28
+    cos, sin = angle.cos(), angle.sin()
+    weights = torch.zeros(B, hkv, 64, device=dev)
+    n = torch.zeros(B, dtype=torch.int32, device=dev)
+    history = torch.zeros(B, 80, dtype=torch.int32)
+
+    def append(counts, positions):
+        N = sum(counts)
+        q, k, v = (torch.randn(N, h, D, generator=g).half() for h in (hq, hkv, hkv))
+        slots, i = torch.empty(N, dtype=torch.int64), 0
+        for b, c in enumerate(counts):
+            for t in range(int(n[b]), int(n[b]) + c):
+                slots[i] = int(tables[b, t // page]) * page + t % page
+                i += 1
+        pos = torch.tensor(positions, dtype=torch.int32)
+        out = ops.rope_paged_append(q.cuda(), k.cuda(), v.cuda(), cos.cuda(), sin.cuda(), pos.cuda(), slots.cuda(), kc, vc)
+        n.add_(torch.tensor(counts, dtype=torch.int32, device=dev))
+        return out
+
+    append(lens, [t for c in lens for t in range(c)])
+    at = list(lens)
+    for step in range(8):
+        q = append([1, 1], at)
+        at = [a + 1 for a in at]
+        before = weights.cpu().double()
+        out, sums, tol = _check_attention(q, kc, vc, tables, n.cpu(), D, torch.float16, weights=weights)
+        for (b, kv), row in sums.items():
+            for t, x in row.items():
+                want = float(before[b, kv, t]) + x
+                assert abs(float(weights[b, kv, t]) - want) <= tol * x + 2 * U * want
+        logits = (torch.randn(B, V, generator=g) * 3)
+        history[:, step] = torch.randint(0, V, (B,), generator=g, dtype=torch.int32)
+        _check_logits(logits, dict(history=history, history_lens=torch.full((B,), step + 1, dtype=torch.int32),
+                                   repetition=torch.full((B,), 1.2), presence=torch.full((B,), 0.5)))
+        if step == 3:
+            kept_ref = oracle.decode_evict(weights.cpu(), n.cpu(), 24, 6, 2, 64)
+            w0 = weights.cpu().clone()
+            kept, new = ops.kv_evict(kc, vc, tables.cuda(), n, weights, 24, 6, sink=2)
+            for b in range(B):
+                for h in range(hkv):
+                    rows = kept_ref[b][h]
+                    assert kept[b, h, :len(rows)].tolist() == rows
+                    assert torch.equal(weights[b, h, :len(rows)].cpu(), w0[b, h, rows])
+            n = new
+            assert n.tolist() == [24, 24]
+            assert bool((weights[:, :, 24:41] == 0).all())

@@ -38,6 +38,8 @@ constexpr int kUnit = 16;      // tokens per unit
 constexpr int kStages = 3;     // units in flight per warp
 constexpr int kWarps = 4;      // warps per CTA
 constexpr int kThreads = kWarps * 32;
+constexpr int kStart = 4;      // cost of starting a segment, in units
+constexpr int kMinRun = 4;     // least points of a run
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct AttnParams {
@@ -50,12 +52,14 @@ struct AttnParams {
   float4* partials;         // [2 warps][NT][D/16][32]
   float4* stats;            // [2 warps][NT][4]: m, l of heads 2c, 2c+1 (log2 units)
   float* scores;            // [B, Hq, score_stride], log2 units, when weights are wanted
-  float2* head_stats;       // [B, Hq]: final m, l, when weights are wanted
+  float2* head_stats;       // [B, Hq]: m, l of heads that were not split, when weights are wanted
   const float* win;
   float* wout;
   int64_t q_sb, q_sh, table_stride, win_sb, win_sh, wout_sb, wout_sh, score_stride;
   int B, hq, hkv, group, tiles, rows;  // tiles of `rows` query heads per kv head
   int num_pages, capacity, window, warps;
+  bool whole_units;  // the page size is a multiple of kUnit
+  int join_ctas;  // CTAs per (b, kv head) that join
   PageDivisor page;
   float score_scale;          // scale * log2(e), or scale / softcap when scores are capped
   float softcap;
@@ -76,15 +80,20 @@ __device__ __forceinline__ Span span_of(const AttnParams& p, int b) {
   return s;
 }
 
-// The units of all sequences before `b`, and of the whole batch, per (kv
-// head, tile); a whole warp calls it.
-__device__ __forceinline__ void unit_sums(const AttnParams& p, int b, int64_t* before, int64_t* all) {
+// The batch's work as a line: each segment, one (sequence, kv head, tile) with
+// visible tokens, is kStart points for starting it (its queries, its output)
+// followed by one point per unit. Runs are equal pieces of this line.
+__device__ __forceinline__ int cost_of(const Span& s) { return s.u1 > s.u0 ? s.u1 - s.u0 + kStart : 0; }
+
+// Points per (kv head, tile) of the sequences before `b`, and of all of them;
+// a whole warp calls it.
+__device__ __forceinline__ void line_sums(const AttnParams& p, int b, int64_t* before, int64_t* all) {
   const int lane = threadIdx.x & 31;
   int64_t lo = 0, sum = 0;
   for (int i = lane; i < p.B; i += 32) {
-    const Span s = span_of(p, i);
-    sum += s.u1 - s.u0;
-    if (i < b) lo += s.u1 - s.u0;
+    const int cost = cost_of(span_of(p, i));
+    sum += cost;
+    if (i < b) lo += cost;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
@@ -94,6 +103,30 @@ __device__ __forceinline__ void unit_sums(const AttnParams& p, int b, int64_t* b
   *before = lo;
   *all = sum;
 }
+
+// Quotient of non-negative values; nearly always both fit 32 bits, where the
+// division takes a fifth of the time.
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+  return a / b;
+}
+
+// The line of `total` points is cut into `count` runs; the first `longer` of
+// them have len + 1 points, the others len.
+struct Runs {
+  int64_t count, len, longer;
+  __device__ __forceinline__ Runs(const AttnParams& p, int64_t total) {
+    const int64_t most = total / kMinRun;
+    count = most < 1 ? 1 : (most < p.warps ? most : p.warps);
+    len = quotient(total, count);
+    longer = total - len * count;
+  }
+  __device__ __forceinline__ int64_t begin(int64_t w) const { return w * len + (w < longer ? w : longer); }
+  __device__ __forceinline__ int64_t holding(int64_t x) const {
+    const int64_t bound = longer * (len + 1);
+    return x < bound ? quotient(x, len + 1) : longer + quotient(x - bound, len);
+  }
+};
 
 // A position in the batch's order of units: sequence, (kv head, tile), unit.
 struct Cursor {
@@ -114,36 +147,42 @@ struct Cursor {
   }
 };
 
-__device__ __forceinline__ Cursor find_unit(const AttnParams& p, int64_t at) {
+// The first unit at or after point `at` of the line, and how many units come
+// before it; a whole warp calls it. Past the end of the line c.b is p.B.
+__device__ __forceinline__ Cursor find_unit(const AttnParams& p, int64_t at, int64_t* units_before) {
   const int lane = threadIdx.x & 31;
   const int heads = p.hkv * p.tiles;
-  Cursor c{0, 0, 0, {0, 0, 0, 0}};
+  const int64_t point = at;
+  int64_t segments = 0;  // before the 32 sequences in hand
+  Cursor c{p.B, 0, 0, {0, 0, 0, 0}};
   for (int b0 = 0; b0 < p.B; b0 += 32) {
     const int b = b0 + lane;
-    int64_t mine = 0;
-    if (b < p.B) {
-      const Span s = span_of(p, b);
-      mine = static_cast<int64_t>(s.u1 - s.u0) * heads;
-    }
+    const int64_t mine = b < p.B ? static_cast<int64_t>(cost_of(span_of(p, b))) * heads : 0;
     int64_t incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int64_t t = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += t;
     }
+    const uint32_t filled = __ballot_sync(0xffffffffu, mine > 0);
     const uint32_t past = __ballot_sync(0xffffffffu, at < incl);
     if (past != 0) {
       const int src = __ffs(past) - 1;
       const int64_t rest = at - __shfl_sync(0xffffffffu, incl - mine, src);
       c.b = b0 + src;
       c.s = span_of(p, c.b);
-      const int per = c.s.u1 - c.s.u0;
-      c.hx = static_cast<int>(rest / per);
-      c.u = c.s.u0 + static_cast<int>(rest % per);
+      const int cost = cost_of(c.s);
+      c.hx = static_cast<int>(quotient(rest, cost));
+      const int in = static_cast<int>(rest - static_cast<int64_t>(c.hx) * cost);
+      c.u = c.s.u0 + (in > kStart ? in - kStart : 0);
+      segments += static_cast<int64_t>(__popc(filled & ((1u << src) - 1u))) * heads + c.hx;
+      *units_before = point - in - segments * kStart + (c.u - c.s.u0);
       return c;
     }
+    segments += static_cast<int64_t>(__popc(filled)) * heads;
     at -= __shfl_sync(0xffffffffu, incl, 31);
   }
+  *units_before = point - at - segments * kStart;
   return c;
 }
 
@@ -240,55 +279,83 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? 2 : 4)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t ring = smem_u32(smem) + warp * (kStages * 2 * kHalf);
 
-  pdl_launch_dependents();
+  // Released only here: the join kernel reads the lengths before its own wait,
+  // so everything launched before this grid has to be complete by then.
   pdl_wait();
+  pdl_launch_dependents();
 
-  int64_t unused, per_head;
-  unit_sums(p, 0, &unused, &per_head);
+  int64_t unused, per_head, units0, units1;
+  line_sums(p, 0, &unused, &per_head);
   const int64_t total = per_head * p.hkv * p.tiles;
-  const int64_t nw = total < p.warps ? total : p.warps;
+  const Runs runs(p, total);
   // Neighbouring runs go to different CTAs, so a small batch spreads over the SMs.
   const int64_t w = static_cast<int64_t>(warp) * gridDim.x + blockIdx.x;
-  if (w >= nw) return;
-  const int64_t first = w * total / nw, last = (w + 1) * total / nw;
-  const int n = static_cast<int>(last - first);
-
-  Cursor ld = find_unit(p, first);
+  if (w >= runs.count) return;
+  Cursor ld = find_unit(p, runs.begin(w), &units0);
+  find_unit(p, runs.begin(w + 1), &units1);
+  const int n = static_cast<int>(units1 - units0);
+  if (n == 0) return;
   Cursor c = ld;
   uint64_t masks = 0;  // 16 validity bits per unit in flight, newest in the low bits
 
-  // Lane r < 16 finds the address of key row r of the unit, lane 16 + r that
-  // of value row r; the copies fetch them by shuffle.
   auto issue = [&](int stage, bool any) {
     uint32_t valid_bits = 0;
     if (any) {
-      const int r = lane & 15;
-      const int t = ld.u * kUnit + r;
-      bool valid = t >= ld.s.lo && t < ld.s.len;
-      const PagedCache& cache = lane < 16 ? p.k : p.v;
-      int64_t off = 0;
-      if (valid) {
-        const uint32_t block = page_of(p.page, t);
-        const int page = p.tables[ld.b * p.table_stride + block];
-        valid = page >= 0 && page < p.num_pages;
-        if (valid) {
-          off = page * cache.page_stride + (ld.hx / p.tiles) * cache.head_stride +
-                static_cast<int64_t>(t - block * p.page.size) * cache.token_stride;
-        }
-      }
-      const uint16_t* src = static_cast<const uint16_t*>(cache.base) + off;
-      valid_bits = __ballot_sync(0xffffffffu, valid) & 0xffffu;
       const int chunk = lane % kChunks;
       const uint32_t base = ring + stage * (2 * kHalf);
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
+      const int64_t head = ld.hx / p.tiles;
+      const int t0 = ld.u * kUnit;
+      if (p.whole_units) {
+        // A unit lies in one page: one table entry, rows a constant stride apart.
+        const uint32_t block = page_of(p.page, t0);
+        const int page = p.tables[ld.b * p.table_stride + block];
+        if (page >= 0 && page < p.num_pages) {
+          const int a = ld.s.lo - t0, z = ld.s.len - t0;  // rows [a, z) are visible
+          valid_bits = (z >= 16 ? 0xffffu : (1u << z) - 1u) & (a > 0 ? ~0u << a : ~0u);
+        }
+        const int64_t at = t0 - static_cast<int64_t>(block) * p.page.size + lane / kChunks;
+        const bool in = valid_bits != 0;
+        const char* ks = static_cast<const char*>(p.k.base) + chunk * 16 +
+                         (in ? 2 * (page * p.k.page_stride + head * p.k.head_stride + at * p.k.token_stride) : 0);
+        const char* vs = static_cast<const char*>(p.v.base) + chunk * 16 +
+                         (in ? 2 * (page * p.v.page_stride + head * p.v.head_stride + at * p.v.token_stride) : 0);
+        const int64_t kstep = in ? 2 * kRowsPerCopy * p.k.token_stride : 0;
+        const int64_t vstep = in ? 2 * kRowsPerCopy * p.v.token_stride : 0;
 #pragma unroll
         for (int i = 0; i < kCopies; ++i) {
           const int row = i * kRowsPerCopy + lane / kChunks;
-          const uint16_t* rsrc = reinterpret_cast<const uint16_t*>(
-              __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), half * 16 + row));
-          cp_async16(base + half * kHalf + row * kRowBytes + ((chunk ^ (row & 7)) << 4), rsrc + chunk * 8,
-                     (valid_bits >> row) & 1);
+          const uint32_t dst = base + row * kRowBytes + ((chunk ^ (row & 7)) << 4);
+          cp_async16(dst, ks + i * kstep, (valid_bits >> row) & 1);
+          cp_async16(dst + kHalf, vs + i * vstep, (valid_bits >> row) & 1);
+        }
+      } else {
+        // Lane r < 16 finds the address of key row r of the unit, lane 16 + r
+        // that of value row r; the copies fetch them by shuffle.
+        const int t = t0 + (lane & 15);
+        bool valid = t >= ld.s.lo && t < ld.s.len;
+        const PagedCache& cache = lane < 16 ? p.k : p.v;
+        int64_t off = 0;
+        if (valid) {
+          const uint32_t block = page_of(p.page, t);
+          const int page = p.tables[ld.b * p.table_stride + block];
+          valid = page >= 0 && page < p.num_pages;
+          if (valid) {
+            off = page * cache.page_stride + head * cache.head_stride +
+                  static_cast<int64_t>(t - block * p.page.size) * cache.token_stride;
+          }
+        }
+        const uint16_t* src = static_cast<const uint16_t*>(cache.base) + off;
+        valid_bits = __ballot_sync(0xffffffffu, valid) & 0xffffu;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+#pragma unroll
+          for (int i = 0; i < kCopies; ++i) {
+            const int row = i * kRowsPerCopy + lane / kChunks;
+            const uint16_t* rsrc = reinterpret_cast<const uint16_t*>(
+                __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), half * 16 + row));
+            cp_async16(base + half * kHalf + row * kRowBytes + ((chunk ^ (row & 7)) << 4), rsrc + chunk * 8,
+                       (valid_bits >> row) & 1);
+          }
         }
       }
       ld.next(p);
@@ -479,125 +546,189 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? 2 : 4)
   }
 }
 
-// One CTA per (sequence, kv head, tile): joins the pieces that the runs left
-// when the segment was split, and writes zeros where no token is visible.
-// Warps take fragments of 16 d x 8 heads; spare warps share the pieces of one
-// fragment and add up in shared memory in a fixed order.
+// A split (sequence, kv head, tile): the runs [w0, w1] hold its pieces. Only
+// the first run can have begun before it, so the first piece is that run's
+// last one unless the run starts with it; the other pieces come first.
+struct Pieces {
+  int64_t w0, first_slot;
+  int count;  // 0: one run had it all
+  __device__ __forceinline__ int64_t slot(int i) const { return i == 0 ? first_slot : (w0 + i) * 2; }
+};
+__device__ __forceinline__ Pieces pieces_of(const AttnParams& p, int64_t before, int64_t all, int hx, int per) {
+  const int heads = p.hkv * p.tiles;
+  const int64_t total = all * heads;
+  const Runs runs(p, total);
+  const int64_t s0 = before * heads + static_cast<int64_t>(hx) * (per + kStart);  // the segment's start
+  const int64_t u0 = s0 + kStart;                                                  // its first unit
+  const int64_t w0 = runs.holding(u0), w1 = runs.holding(u0 + per - 1);
+  return Pieces{w0, w0 * 2 + (runs.begin(w0) >= s0 ? 0 : 1), w0 == w1 ? 0 : static_cast<int>(w1 - w0 + 1)};
+}
+
+// The second kernel, CTAs (b, kv head) x y. y < join_ctas: join the pieces of
+// split segments (and write zeros where no token is visible); each warp takes
+// one fragment of 16 d x 8 heads and every kParts-th piece, and the warps of a
+// fragment add up in shared memory in a fixed order. Other y, when the weights
+// are wanted: kWeightTokens tokens of
+//   weights_out[t] = weights_in[t] + sum_h exp2(s[h, t] - m[h]) / l[h].
 constexpr int kJoinWarps = 16;
+constexpr int kJoinThreads = kJoinWarps * 32;
+constexpr int kWeightTokens = 1024;
+constexpr int kWeightSteps = kWeightTokens / kJoinThreads;
 
 template <bool kBf16, int D, int NT, bool kScores>
-__global__ void __launch_bounds__(kJoinWarps * 32) paged_attention_join_kernel(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(kJoinThreads) paged_attention_join_kernel(const __grid_constant__ AttnParams p) {
   constexpr int kFrags = NT * (D / 16);
-  constexpr int kParts = kJoinWarps / kFrags;
   __shared__ float4 acc[kJoinWarps][32];
   __shared__ float4 sums[kJoinWarps][4];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  pdl_launch_dependents();
-  pdl_wait();
-  const int heads = p.hkv * p.tiles;
-  const int b = blockIdx.x / heads, hx = blockIdx.x % heads;
-  const int tile = hx % p.tiles;
-  const int h0 = (hx / p.tiles) * p.group + tile * p.rows;
-  const int nrows = p.group - tile * p.rows < p.rows ? p.group - tile * p.rows : p.rows;
-  uint16_t* head0 = p.out + (static_cast<int64_t>(b) * p.hq + h0) * D;
-  const Span s = span_of(p, b);
-  const int per = s.u1 - s.u0;
-  if (per == 0) {
-    uint32_t* dst = reinterpret_cast<uint32_t*>(head0);
-    for (int i = threadIdx.x; i < nrows * D / 2; i += blockDim.x) dst[i] = 0u;
-    return;
-  }
-  int64_t before, all;
-  unit_sums(p, b, &before, &all);
-  const int64_t total = all * heads;
-  const int64_t nw = total < p.warps ? total : p.warps;
-  const int64_t s0 = before * heads + static_cast<int64_t>(hx) * per;
-  // The run that holds unit x is the largest w with w * total / nw <= x.
-  const int64_t w0 = ((s0 + 1) * nw - 1) / total, w1 = ((s0 + per) * nw - 1) / total;
-  if (w0 == w1) return;
-  const int pieces = static_cast<int>(w1 - w0 + 1);
-  // Piece i's slot: only the first run can have begun before the segment.
-  const int64_t head_slot = w0 * 2 + (w0 * total / nw == s0 ? 0 : 1);
-  auto slot_of = [&](int i) { return i == 0 ? head_slot : (w0 + i) * 2; };
-
-  const int part = warp / kFrags, frag = warp % kFrags, nt = frag / (D / 16);
-  float m0 = -INFINITY, m1 = -INFINITY;
-  for (int i = lane >> 2; i < pieces; i += 8) {
-    const float4 st = p.stats[(slot_of(i) * NT + nt) * 4 + (lane & 3)];
-    m0 = fmaxf(m0, st.x);
-    m1 = fmaxf(m1, st.z);
-  }
-#pragma unroll
-  for (int d = 4; d < 32; d <<= 1) {
-    m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, d));
-    m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, d));
-  }
-  const float r0 = safe_max(m0), r1 = safe_max(m1);
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  float l0 = 0.f, l1 = 0.f;
-#pragma unroll 4
-  for (int i = part; i < pieces; i += kParts) {
-    const int64_t slot = slot_of(i) * NT + nt;
-    const float4 st = p.stats[slot * 4 + (lane & 3)];
-    const float4 x = p.partials[(slot * (D / 16) + frag % (D / 16)) * 32 + lane];
-    const float a0 = ex2_approx(st.x - r0), a1 = ex2_approx(st.z - r1);
-    l0 = fmaf(st.y, a0, l0);
-    l1 = fmaf(st.w, a1, l1);
-    o.x = fmaf(x.x, a0, o.x);
-    o.y = fmaf(x.y, a1, o.y);
-    o.z = fmaf(x.z, a0, o.z);
-    o.w = fmaf(x.w, a1, o.w);
-  }
-  if (kParts > 1) {
-    acc[warp][lane] = o;
-    if (lane < 4) sums[warp][lane] = make_float4(l0, l1, 0.f, 0.f);
-    __syncthreads();
-    if (part > 0) return;
-#pragma unroll
-    for (int k = 1; k < kParts; ++k) {
-      const float4 x = acc[k * kFrags + frag][lane], y = sums[k * kFrags + frag][lane & 3];
-      o.x += x.x;
-      o.y += x.y;
-      o.z += x.z;
-      o.w += x.w;
-      l0 += y.x;
-      l1 += y.y;
-    }
-  }
-  const float i0 = inv_sum(l0), i1 = inv_sum(l1);
-  const float t[4] = {o.x * i0, o.y * i1, o.z * i0, o.w * i1};
-  store_out_tile<kBf16>(p, t, head0, D, nt, frag % (D / 16), nrows);
-  if (kScores && frag % (D / 16) == 0 && lane < 4) {
-    float2* hs = p.head_stats + static_cast<int64_t>(b) * p.hq + h0;
-    const int col = nt * 8 + lane * 2;
-    if (col < nrows) hs[col] = make_float2(m0, l0);
-    if (col + 1 < nrows) hs[col + 1] = make_float2(m1, l1);
-  }
-}
-
-// weights_out[b, kv, t] = weights_in[b, kv, t] + sum_h exp2(s[h, t] - m[h]) / l[h].
-constexpr int kWeightThreads = 256;
-constexpr int kWeightTokens = 1024;
-
-__global__ void __launch_bounds__(kWeightThreads) paged_attention_weights_kernel(const __grid_constant__ AttnParams p) {
-  pdl_launch_dependents();
-  pdl_wait();
   const int b = blockIdx.x / p.hkv, kv = blockIdx.x % p.hkv;
   const Span s = span_of(p, b);
-  const int64_t head = static_cast<int64_t>(b) * p.hq + static_cast<int64_t>(kv) * p.group;
-  const float* in = p.win + b * p.win_sb + kv * p.win_sh;
-  float* out = p.wout + b * p.wout_sb + kv * p.wout_sh;
-  const int begin = blockIdx.y * kWeightTokens;
-  const int end = s.len - begin > kWeightTokens ? begin + kWeightTokens : s.len;
-  for (int t = begin + threadIdx.x; t < end; t += kWeightThreads) {
-    float sum = 0.f;
-    if (t >= s.lo) {
-      for (int h = 0; h < p.group; ++h) {
-        const float2 st = p.head_stats[head + h];
-        sum = fmaf(ex2_approx(p.scores[(head + h) * p.score_stride + t] - safe_max(st.x)), inv_sum(st.y), sum);
+  const int per = s.u1 - s.u0;
+  int64_t before, all;
+  line_sums(p, b, &before, &all);
+  pdl_wait();
+  pdl_launch_dependents();
+
+  if (!kScores || blockIdx.y < p.join_ctas) {
+    const int frags = kFrags / p.join_ctas;  // per CTA
+    const int parts = kJoinWarps / frags;
+    const int part = warp / frags, frag = blockIdx.y * frags + warp % frags;
+    const int nt = frag / (D / 16), dt = frag % (D / 16);
+    for (int tile = 0; tile < p.tiles; ++tile) {
+      const int h0 = kv * p.group + tile * p.rows;
+      const int nrows = p.group - tile * p.rows < p.rows ? p.group - tile * p.rows : p.rows;
+      uint16_t* head0 = p.out + (static_cast<int64_t>(b) * p.hq + h0) * D;
+      if (per == 0) {
+        uint32_t* dst = reinterpret_cast<uint32_t*>(head0);
+        for (int i = blockIdx.y * kJoinThreads + threadIdx.x; i < nrows * D / 2; i += p.join_ctas * kJoinThreads) dst[i] = 0u;
+        continue;
+      }
+      const Pieces pc = pieces_of(p, before, all, kv * p.tiles + tile, per);
+      if (pc.count == 0) continue;
+      float m0 = -INFINITY, m1 = -INFINITY;
+      for (int i = lane >> 2; i < pc.count; i += 8) {
+        const float4 st = p.stats[(pc.slot(i) * NT + nt) * 4 + (lane & 3)];
+        m0 = fmaxf(m0, st.x);
+        m1 = fmaxf(m1, st.z);
+      }
+#pragma unroll
+      for (int d = 4; d < 32; d <<= 1) {
+        m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, d));
+        m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, d));
+      }
+      const float r0 = safe_max(m0), r1 = safe_max(m1);
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+      float l0 = 0.f, l1 = 0.f;
+#pragma unroll 4
+      for (int i = part; i < pc.count; i += parts) {
+        const int64_t slot = pc.slot(i) * NT + nt;
+        const float4 st = p.stats[slot * 4 + (lane & 3)];
+        const float4 x = p.partials[(slot * (D / 16) + dt) * 32 + lane];
+        const float a0 = ex2_approx(st.x - r0), a1 = ex2_approx(st.z - r1);
+        l0 = fmaf(st.y, a0, l0);
+        l1 = fmaf(st.w, a1, l1);
+        o.x = fmaf(x.x, a0, o.x);
+        o.y = fmaf(x.y, a1, o.y);
+        o.z = fmaf(x.z, a0, o.z);
+        o.w = fmaf(x.w, a1, o.w);
+      }
+      if (parts > 1) {
+        __syncthreads();  // the last tile's sums have been read
+        acc[warp][lane] = o;
+        if (lane < 4) sums[warp][lane] = make_float4(l0, l1, 0.f, 0.f);
+        __syncthreads();
+        if (part > 0) continue;
+        for (int k = 1; k < parts; ++k) {
+          const float4 x = acc[k * frags + warp][lane], y = sums[k * frags + warp][lane & 3];
+          o.x += x.x;
+          o.y += x.y;
+          o.z += x.z;
+          o.w += x.w;
+          l0 += y.x;
+          l1 += y.y;
+        }
+      }
+      const float i0 = inv_sum(l0), i1 = inv_sum(l1);
+      const float t[4] = {o.x * i0, o.y * i1, o.z * i0, o.w * i1};
+      store_out_tile<kBf16>(p, t, head0, D, nt, dt, nrows);
+    }
+    return;
+  }
+
+  if constexpr (kScores) {
+    float2* stat = reinterpret_cast<float2*>(&sums[0][0]);  // 16 heads: reference point, 1 / l
+    const float* in = p.win + b * p.win_sb + kv * p.win_sh;
+    float* out = p.wout + b * p.wout_sb + kv * p.wout_sh;
+    const int begin = (blockIdx.y - p.join_ctas) * kWeightTokens + threadIdx.x;
+    if (begin - static_cast<int>(threadIdx.x) >= s.len) return;
+    float w[kWeightSteps];
+#pragma unroll
+    for (int i = 0; i < kWeightSteps; ++i) {
+      const int t = begin + i * kJoinThreads;
+      w[i] = t < s.len ? in[t] : 0.f;
+    }
+    for (int tile = 0; tile < p.tiles; ++tile) {
+      const int h0 = kv * p.group + tile * p.rows;
+      const int nrows = p.group - tile * p.rows < p.rows ? p.group - tile * p.rows : p.rows;
+      const int64_t head = static_cast<int64_t>(b) * p.hq + h0;
+      const Pieces pc = pieces_of(p, before, all, kv * p.tiles + tile, per);
+      __syncthreads();
+      if (warp < NT) {
+        // Lane quads add up the pieces of two heads each.
+        const int col = warp * 8 + (lane & 3) * 2;
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+        if (pc.count == 0) {
+          for (int j = 0; j < 2; ++j) {
+            if (col + j < nrows) {
+              const float2 st = p.head_stats[head + col + j];
+              m[j] = st.x;
+              l[j] = st.y;
+            }
+          }
+        } else {
+          for (int i = lane >> 2; i < pc.count; i += 8) {
+            const float4 st = p.stats[(pc.slot(i) * NT + warp) * 4 + (lane & 3)];
+            m[0] = fmaxf(m[0], st.x);
+            m[1] = fmaxf(m[1], st.z);
+          }
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) {
+            m[0] = fmaxf(m[0], __shfl_xor_sync(0xffffffffu, m[0], d));
+            m[1] = fmaxf(m[1], __shfl_xor_sync(0xffffffffu, m[1], d));
+          }
+          for (int i = lane >> 2; i < pc.count; i += 8) {
+            const float4 st = p.stats[(pc.slot(i) * NT + warp) * 4 + (lane & 3)];
+            l[0] = fmaf(st.y, ex2_approx(st.x - safe_max(m[0])), l[0]);
+            l[1] = fmaf(st.w, ex2_approx(st.z - safe_max(m[1])), l[1]);
+          }
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) {
+            l[0] += __shfl_xor_sync(0xffffffffu, l[0], d);
+            l[1] += __shfl_xor_sync(0xffffffffu, l[1], d);
+          }
+        }
+        if (lane < 4) {
+          stat[col] = make_float2(safe_max(m[0]), inv_sum(l[0]));
+          stat[col + 1] = make_float2(safe_max(m[1]), inv_sum(l[1]));
+        }
+      }
+      __syncthreads();
+#pragma unroll 4
+      for (int h = 0; h < nrows; ++h) {
+        const float* row = p.scores + (head + h) * p.score_stride;
+        const float2 st = stat[h];
+#pragma unroll
+        for (int i = 0; i < kWeightSteps; ++i) {
+          const int t = begin + i * kJoinThreads;
+          if (t >= s.lo && t < s.len) w[i] = fmaf(ex2_approx(row[t] - st.x), st.y, w[i]);
+        }
       }
     }
-    out[t] = in[t] + sum;
+#pragma unroll
+    for (int i = 0; i < kWeightSteps; ++i) {
+      const int t = begin + i * kJoinThreads;
+      if (t < s.len) out[t] = w[i];
+    }
   }
 }
 
@@ -653,15 +784,10 @@ int launch_attention(const AttnParams& p, const Plan& pl, cudaStream_t stream) {
   if (rc != NESO_OK) return rc;
   cudaError_t e = launch_pdl(kern, dim3(pl.ctas), dim3(kThreads), smem, stream, p);
   if (e != cudaSuccess) return cuda_fail(e, "paged_attention launch");
-  e = launch_pdl(paged_attention_join_kernel<kBf16, D, NT, kScores>, dim3(p.B * p.hkv * p.tiles),
-                 dim3(kJoinWarps * 32), 0, stream, p);
+  const int64_t chunks = kScores ? (pl.capacity + kWeightTokens - 1) / kWeightTokens : 0;
+  e = launch_pdl(paged_attention_join_kernel<kBf16, D, NT, kScores>,
+                 dim3(p.B * p.hkv, static_cast<unsigned>(p.join_ctas + chunks)), dim3(kJoinThreads), 0, stream, p);
   if (e != cudaSuccess) return cuda_fail(e, "paged_attention join launch");
-  if (kScores) {
-    const int64_t chunks = (pl.capacity + kWeightTokens - 1) / kWeightTokens;
-    e = launch_pdl(paged_attention_weights_kernel, dim3(p.B * p.hkv, static_cast<unsigned>(chunks)),
-                   dim3(kWeightThreads), 0, stream, p);
-    if (e != cudaSuccess) return cuda_fail(e, "paged_attention weights launch");
-  }
   return ok();
 }
 
@@ -739,8 +865,8 @@ int neso_paged_attention(const void* q, const void* k_cache, const void* v_cache
                 static_cast<long long>(workspace == nullptr ? 0 : workspace_bytes), static_cast<long long>(pl.bytes));
   }
   if (!aligned16(workspace)) return fail(NESO_ERR_MISALIGNED, "workspace is not 16-byte aligned");
-  if (weights_out != nullptr && (pl.capacity + kWeightTokens - 1) / kWeightTokens > 65535) {
-    return fail(NESO_ERR_UNSUPPORTED, "weights are limited to tables of 65535 x %d tokens", kWeightTokens);
+  if (weights_out != nullptr && (pl.capacity + kWeightTokens - 1) / kWeightTokens > 65000) {
+    return fail(NESO_ERR_UNSUPPORTED, "weights are limited to tables of 65000 x %d tokens", kWeightTokens);
   }
   p.q = static_cast<const uint16_t*>(q);
   p.tables = block_tables;
@@ -772,6 +898,11 @@ int neso_paged_attention(const void* q, const void* k_cache, const void* v_cache
   p.capacity = static_cast<int>(pl.capacity);
   p.window = window;
   p.warps = pl.warps;
+  p.whole_units = page_size % kUnit == 0;
+  // With few (sequence, kv head) pairs each has many pieces and the SMs are
+  // idle: a CTA per fragment then.
+  const int frags = pl.nt * (D / 16);
+  p.join_ctas = static_cast<int64_t>(B) * Hkv * frags <= 2 * sm_count() ? frags : 1;
   p.page = page_divisor(static_cast<uint32_t>(page_size));
   p.score_scale = softcap > 0.f ? scale / softcap : scale * kLog2e;
   p.softcap = softcap;

@@ -5,13 +5,15 @@
 // their slots. One pass: every input byte is read once and every output byte
 // written once, so HBM bounds it (launch latency for a few tokens).
 //
-// kv_evict: for each (sequence, kv head) the kept set is found by a radix
-// selection on the weights' bits and the kept rows are moved together, in order.
-// A cluster of CTAs owns one (sequence, kv head): it counts digits in its
-// CTAs' shared memory, ranks the kept tokens by a scan, and moves the rows in
-// steps, all CTAs side by side. Moving in place is safe because row j comes
-// from row src_j >= j: when a step's rows are all in registers (a cluster
-// barrier), the rows that it overwrites are not the source of any later step.
+// kv_evict, first kernel: for each (sequence, kv head) the kept set is found by
+// a radix selection on the weights' bits. Up to kShortLen tokens one CTA does
+// it in registers and shared memory; longer sequences are counted by a cluster
+// through its shared memory. Second kernel: the kept rows move together, in
+// order. Under a table of their own they move independently of each other. In
+// place, a cluster moves the rows of one (sequence, kv head) a step at a time:
+// row j comes from row src_j >= j, so when all rows of a step are in shared
+// memory (a cluster barrier), the rows that it overwrites are not the source
+// of any later step, and later steps may already be on their way in.
 #include <cooperative_groups.h>
 
 #include "paged.h"
@@ -33,7 +35,8 @@ struct RopeParams {
   int64_t q_sn, q_sh, k_sn, k_sh, v_sn, v_sh, slot_count;
   int N, hq, hkv, D, half, table_rows, axes;
   int section_end[kMaxAxes];
-  PageDivisor page;
+  int group;  // tokens per CTA
+  PageDivisor page, per_head, heads;  // heads: of q, k and v
 };
 
 template <bool kBf16>
@@ -71,74 +74,133 @@ __device__ __forceinline__ void store_vec(uint16_t* p, const Vec<N>& r) {
 }
 
 constexpr int kRopeThreads = 256;
+constexpr int kRopeBatch = 3;    // items whose loads a thread has in flight
+constexpr int kRopeTokens = 4;   // tokens per CTA when there are many
+constexpr int kMaxRopeDim = 1024;
 
-// One CTA per token (grid-stride). A work item is kVec rotated pairs of one
-// head, or kVec elements that are copied.
+// A CTA takes p.group tokens. Every head of q, k and v is D / (2 kVec) items
+// of two vectors: a rotated pair, or two that are copied (the rest of a
+// rotated head, and values). The first items are requested before the chain
+// position -> angles, which is walked once per CTA into shared memory.
 template <bool kBf16, int kVec>
 __global__ void __launch_bounds__(kRopeThreads) rope_paged_append_kernel(const __grid_constant__ RopeParams p) {
+  extern __shared__ __align__(16) float angles[];  // [group][2][half]
+  __shared__ int64_t places[kRopeTokens][2];        // element offsets in k_cache and v_cache, or -1
+  const int tid = threadIdx.x;
+  const int n0 = blockIdx.x * p.group;
+  const int tokens = min(p.group, p.N - n0);
+  const int rotated = p.hq + p.hkv, heads = rotated + p.hkv;
+  const int per_head = p.D / (2 * kVec);
+  const int items = tokens * heads * per_head;
   pdl_launch_dependents();
   pdl_wait();
-  const int hv = p.half / kVec, rest = p.D / kVec - 2 * hv, dv = p.D / kVec;
-  const int per_head = hv + rest;
-  const int items = (p.hq + p.hkv) * per_head + p.hkv * dv;
-  for (int n = blockIdx.x; n < p.N; n += gridDim.x) {
-    const int64_t slot = p.slots[n];
-    const bool pad = slot < 0 || slot >= p.slot_count;
-    uint16_t* q_row = p.q_out + static_cast<int64_t>(n) * p.hq * p.D;
-    if (pad) {
-      Vec<kVec> zero;
+
+  struct Item {
+    int n, h, d, second;  // token, head, first element, distance of the second
+    bool turned;
+  };
+  auto item_at = [&](int i) {
+    Item it;
+    const int hn = static_cast<int>(page_of(p.per_head, i));
+    const int c = i - hn * per_head;
+    it.n = static_cast<int>(page_of(p.heads, hn));
+    it.h = hn - it.n * heads;
+    const int turn = it.h < rotated ? p.half : 0;  // pairs that turn
+    it.turned = c * kVec < turn;
+    it.d = it.turned ? c * kVec : c * kVec + turn;
+    it.second = it.turned ? p.half : p.D / 2 - turn;
+    return it;
+  };
+  auto source = [&](const Item& it) {
+    const int64_t n = n0 + it.n;
+    if (it.h < p.hq) return p.q + n * p.q_sn + it.h * p.q_sh + it.d;
+    if (it.h < rotated) return p.k + n * p.k_sn + (it.h - p.hq) * p.k_sh + it.d;
+    return p.v + n * p.v_sn + (it.h - rotated) * p.v_sh + it.d;
+  };
+  Vec<kVec> x[kRopeBatch], y[kRopeBatch];
+  auto request = [&](int i0) {
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) zero.e[i] = 0;
-      for (int i = threadIdx.x; i < p.hq * dv; i += kRopeThreads) store_vec<kVec>(q_row + i * kVec, zero);
-      continue;
+    for (int j = 0; j < kRopeBatch; ++j) {
+      const int i = i0 + j * kRopeThreads;
+      if (i < items) {
+        const Item it = item_at(i);
+        const uint16_t* src = source(it);
+        x[j] = load_vec<kVec>(src);
+        y[j] = load_vec<kVec>(src + it.second);
+      }
     }
-    const int64_t page = slot / p.page.size;
-    const int64_t row = slot - page * p.page.size;
-    uint16_t* kc = static_cast<uint16_t*>(p.kc.base) + page * p.kc.page_stride + row * p.kc.token_stride;
-    uint16_t* vc = static_cast<uint16_t*>(p.vc.base) + page * p.vc.page_stride + row * p.vc.token_stride;
-    for (int i = threadIdx.x; i < items; i += kRopeThreads) {
-      if (i >= (p.hq + p.hkv) * per_head) {
-        const int j = i - (p.hq + p.hkv) * per_head;
-        const int h = j / dv, d = (j % dv) * kVec;
-        store_vec<kVec>(vc + h * p.vc.head_stride + d, load_vec<kVec>(p.v + n * p.v_sn + h * p.v_sh + d));
-        continue;
-      }
-      const int h = i / per_head, c = i % per_head;
-      const uint16_t* src = h < p.hq ? p.q + n * p.q_sn + h * p.q_sh : p.k + n * p.k_sn + (h - p.hq) * p.k_sh;
-      uint16_t* dst = h < p.hq ? q_row + static_cast<int64_t>(h) * p.D : kc + (h - p.hq) * p.kc.head_stride;
-      if (c >= hv) {
-        const int d = 2 * p.half + (c - hv) * kVec;
-        store_vec<kVec>(dst + d, load_vec<kVec>(src + d));
-        continue;
-      }
-      const int d = c * kVec;
-      const Vec<kVec> a = load_vec<kVec>(src + d), b = load_vec<kVec>(src + d + p.half);
-      Vec<kVec> x, y;
+  };
+  request(tid);
+
+  if (tid < tokens) {
+    const int64_t slot = p.slots[n0 + tid];
+    int64_t ko = -1, vo = -1;
+    if (slot >= 0 && slot < p.slot_count) {
+      const int64_t page = p.slot_count <= INT32_MAX ? static_cast<int64_t>(page_of(p.page, static_cast<uint32_t>(slot)))
+                                                     : slot / p.page.size;
+      const int64_t row = slot - page * p.page.size;
+      ko = page * p.kc.page_stride + row * p.kc.token_stride;
+      vo = page * p.vc.page_stride + row * p.vc.token_stride;
+    }
+    places[tid][0] = ko;
+    places[tid][1] = vo;
+  }
+  for (int i = tid; i < tokens * p.half; i += kRopeThreads) {
+    const int n = i / p.half, d = i - n * p.half;
+    int axis = 0;
+    while (axis < p.axes - 1 && d >= p.section_end[axis]) ++axis;
+    const int pos = p.positions[static_cast<int64_t>(axis) * p.N + n0 + n];
+    const bool in = pos >= 0 && pos < p.table_rows;
+    const int64_t at = static_cast<int64_t>(pos) * p.half + d;
+    angles[(2 * n) * p.half + d] = in ? p.cos[at] : __int_as_float(0x7fc00000);
+    angles[(2 * n + 1) * p.half + d] = in ? p.sin[at] : __int_as_float(0x7fc00000);
+  }
+  __syncthreads();
+
+  for (int i0 = tid; i0 < items; i0 += kRopeBatch * kRopeThreads) {
+    if (i0 != tid) request(i0);
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) {
-        int axis = 0;
-        while (axis < p.axes - 1 && d + e >= p.section_end[axis]) ++axis;
-        const int pos = p.positions[static_cast<int64_t>(axis) * p.N + n];
-        float cs = __int_as_float(0x7fc00000), sn = cs;
-        if (pos >= 0 && pos < p.table_rows) {
-          cs = p.cos[static_cast<int64_t>(pos) * p.half + d + e];
-          sn = p.sin[static_cast<int64_t>(pos) * p.half + d + e];
+    for (int j = 0; j < kRopeBatch; ++j) {
+      const int i = i0 + j * kRopeThreads;
+      if (i >= items) break;
+      const Item it = item_at(i);
+      const int64_t ko = places[it.n][0], vo = places[it.n][1];
+      uint16_t* dst;
+      if (it.h < p.hq) {
+        dst = p.q_out + (static_cast<int64_t>(n0 + it.n) * p.hq + it.h) * p.D + it.d;
+        if (ko < 0) {
+#pragma unroll
+          for (int e = 0; e < kVec; ++e) x[j].e[e] = y[j].e[e] = 0;
         }
-        const float u = to_float<kBf16>(a.e[e]), w = to_float<kBf16>(b.e[e]);
-        x.e[e] = from_float<kBf16>(__fsub_rn(__fmul_rn(u, cs), __fmul_rn(w, sn)));
-        y.e[e] = from_float<kBf16>(__fadd_rn(__fmul_rn(u, sn), __fmul_rn(w, cs)));
+      } else {
+        if (ko < 0) continue;
+        dst = it.h < rotated ? static_cast<uint16_t*>(p.kc.base) + ko + (it.h - p.hq) * p.kc.head_stride + it.d
+                             : static_cast<uint16_t*>(p.vc.base) + vo + (it.h - rotated) * p.vc.head_stride + it.d;
       }
-      store_vec<kVec>(dst + d, x);
-      store_vec<kVec>(dst + d + p.half, y);
+      if (it.turned && ko >= 0) {
+        const float* cs = angles + 2 * it.n * p.half + it.d;
+        const float* sn = cs + p.half;
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) {
+          const float u = to_float<kBf16>(x[j].e[e]), w = to_float<kBf16>(y[j].e[e]);
+          x[j].e[e] = from_float<kBf16>(__fsub_rn(__fmul_rn(u, cs[e]), __fmul_rn(w, sn[e])));
+          y[j].e[e] = from_float<kBf16>(__fadd_rn(__fmul_rn(u, sn[e]), __fmul_rn(w, cs[e])));
+        }
+      }
+      store_vec<kVec>(dst, x[j]);
+      store_vec<kVec>(dst + it.second, y[j]);
     }
   }
 }
 
 template <bool kBf16, int kVec>
-int launch_rope(const RopeParams& p, cudaStream_t stream) {
-  const int64_t cap = static_cast<int64_t>(sm_count()) * 64;
-  const unsigned grid = static_cast<unsigned>(p.N < cap ? p.N : cap);
-  cudaError_t e = launch_pdl(rope_paged_append_kernel<kBf16, kVec>, dim3(grid), dim3(kRopeThreads), 0, stream, p);
+int launch_rope(RopeParams p, cudaStream_t stream) {
+  // A token to a CTA while that leaves SMs idle, for the shorter latency.
+  p.group = p.N >= 8 * sm_count() ? kRopeTokens : 1;
+  p.per_head = page_divisor(static_cast<uint32_t>(p.D / (2 * kVec)));
+  const unsigned grid = static_cast<unsigned>((p.N + p.group - 1) / p.group);
+  const size_t smem = static_cast<size_t>(p.group) * 2 * p.half * sizeof(float);
+  cudaError_t e = launch_pdl(rope_paged_append_kernel<kBf16, kVec>, dim3(grid), dim3(kRopeThreads), smem, stream, p);
   return e == cudaSuccess ? ok() : cuda_fail(e, "rope_paged_append launch");
 }
 
@@ -151,14 +213,22 @@ struct EvictParams {
   int32_t *kept, *new_lens;
   int64_t table_stride, out_stride, win_sb, win_sh, wout_sb, wout_sh;
   int hkv, D, budget, recent, sink, num_pages, capacity, out_capacity;
+  int row_shift;  // log2 of the pieces of a K row and a V row, or -1
   PageDivisor page;
 };
 
 constexpr int kEvictThreads = 512;
-constexpr int kEvictCluster = 8;
+constexpr int kEvictWarps = kEvictThreads / 32;
+constexpr int kMaxCluster = 8;
 constexpr int kDigitBits = 8;
 constexpr int kDigits = 1 << kDigitBits;
-constexpr int kMoveRows = 2;  // 16-byte pieces per thread, cache and step
+constexpr int kCopiesOfHist = 8;   // counters of a digit, so that equal digits of a warp collide less
+constexpr int kHistPitch = kDigits + 1;
+constexpr int kItems = 16;         // tokens per thread of a short sequence
+constexpr int kShortLen = kEvictThreads * kItems;
+constexpr int kMoveThreads = 512;
+constexpr int kMoveStages = 4;     // steps of rows in flight, one 16-byte piece per thread and cache each
+constexpr int kMoveBytes = kMoveStages * 2 * kMoveThreads * 16;
 
 // Larger weights get larger keys; NaN the largest; -0 and +0 the same key.
 __device__ __forceinline__ uint32_t weight_key(float w) {
@@ -167,20 +237,97 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-__global__ void __cluster_dims__(kEvictCluster, 1, 1) __launch_bounds__(kEvictThreads)
-    kv_evict_kernel(const __grid_constant__ EvictParams p) {
-  __shared__ int hist[kDigits];
-  __shared__ int total[kDigits];
-  __shared__ int above_of[2];   // this CTA's slice: tokens above the threshold, tokens at it
-  __shared__ int warp_sum[2][kEvictThreads / 32];
-  __shared__ int pick[2];
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+// Execution barrier of the cluster that does not wait for stores on their way
+// to memory (the ordinary one does, microseconds at a time): for steps whose
+// loads have completed and whose stores nobody reads.
+__device__ __forceinline__ void cluster_barrier_relaxed() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+}
+
+struct EvictShared {
+  int hist[kCopiesOfHist * kHistPitch];
+  alignas(16) int total[kDigits];
+  int warp_sum[2][kEvictWarps];
+  int slice[2];  // long sequences: kept for sure and ties of this CTA's slice
+  int pick[3];
+};
+// Short sequences, dynamic shared memory: the weights (padded), then the kept
+// tokens and their weights.
+constexpr int kSelectBytes = (kShortLen + kEvictThreads + kShortLen) * 4;
+
+// Count this thread's digit, in its copy of the histogram.
+__device__ __forceinline__ void count_digit(EvictShared& sh, uint32_t key, uint32_t prefix, int shift) {
+  if (shift == 32 - kDigitBits || ((key ^ prefix) >> (shift + kDigitBits)) == 0) {
+    atomicAdd(&sh.hist[(threadIdx.x % kCopiesOfHist) * kHistPitch + ((key >> shift) & (kDigits - 1))], 1);
+  }
+}
+
+// From total[]: the digit that holds the need-th largest key (pick[0]), how
+// many of its keys are wanted (pick[1]) and how many it has (pick[2]). Warp 0.
+__device__ __forceinline__ void pick_digit(EvictShared& sh, int need) {
+  constexpr int kPer = kDigits / 32;
+  const int lane = threadIdx.x & 31;
+  int mine = 0;  // digits from the largest down, kPer to a lane
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) mine += sh.total[kDigits - 1 - (lane * kPer + j)];
+  int incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += x;
+  }
+  int before = incl - mine;
+  if (before < need && need <= incl) {
+    for (int j = 0; j < kPer; ++j) {
+      const int digit = kDigits - 1 - (lane * kPer + j);
+      if (before + sh.total[digit] >= need) {
+        sh.pick[0] = digit;
+        sh.pick[1] = need - before;
+        sh.pick[2] = sh.total[digit];
+        break;
+      }
+      before += sh.total[digit];
+    }
+  }
+}
+
+// What a selection found: keys above `bound` are kept, and the first `ties`
+// tokens whose key equals it.
+struct Selected {
+  uint32_t bound;
+  int ties;
+};
+
+__global__ void __launch_bounds__(kEvictThreads, 2) kv_select_kernel(const __grid_constant__ EvictParams p) {
+  __shared__ EvictShared sh;
+  extern __shared__ __align__(16) int lists[];
+  int* list = lists;
+  int* kept_bits = lists + kShortLen + kEvictThreads;
   cg::cluster_group cluster = cg::this_cluster();
+  const int ctas = static_cast<int>(cluster.num_blocks());
   const int rank = static_cast<int>(cluster.block_rank());
-  const int seg = blockIdx.x / kEvictCluster;
+  const int seg = blockIdx.x / ctas;
   const int b = seg / p.hkv, h = seg % p.hkv;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  pdl_launch_dependents();
   pdl_wait();
+  pdl_launch_dependents();
+  auto sync_cluster = [&] {
+    if (ctas > 1) {
+      cluster.sync();
+    } else {
+      __syncthreads();
+    }
+  };
 
   int len = p.lens[b];
   len = len < 0 ? 0 : (len > p.capacity ? p.capacity : len);
@@ -188,180 +335,349 @@ __global__ void __cluster_dims__(kEvictCluster, 1, 1) __launch_bounds__(kEvictTh
   const float* win = p.win + b * p.win_sb + h * p.win_sh;
   float* wout = p.wout + b * p.wout_sb + h * p.wout_sh;
   int32_t* kept = p.kept + (static_cast<int64_t>(b) * p.hkv + h) * p.budget;
-
   // Candidates [lo, hi) are ranked; tokens outside are kept.
   const bool all = len <= p.budget;
   const int lo = all ? 0 : p.sink, hi = all ? 0 : len - p.recent;
-  int need = all ? 0 : keep - p.sink - p.recent;  // candidates to keep
-  // This CTA's slice of the whole sequence.
-  const int per = (len + kEvictCluster - 1) / kEvictCluster;
-  const int t0 = min(len, rank * per), t1 = min(len, t0 + per);
+  const int wanted = all ? 0 : keep - p.sink - p.recent;  // candidates to keep
+  const bool is_short = len <= kShortLen;
 
-  // The need-th largest key, digit by digit from the top: `prefix` holds the
-  // digits found so far, `need` how many of the keys that share it are kept.
-  uint32_t prefix = 0;
-  if (need > 0) {
-    for (int shift = 32 - kDigitBits; shift >= 0; shift -= kDigitBits) {
-      for (int i = tid; i < kDigits; i += kEvictThreads) hist[i] = 0;
-      __syncthreads();
-      for (int t = max(t0, lo) + tid; t < min(t1, hi); t += kEvictThreads) {
-        const uint32_t key = weight_key(win[t]);
-        if (shift == 32 - kDigitBits || (key >> (shift + kDigitBits)) == (prefix >> (shift + kDigitBits))) {
-          atomicAdd(&hist[(key >> shift) & (kDigits - 1)], 1);
-        }
-      }
-      cluster.sync();
-      for (int i = tid; i < kDigits; i += kEvictThreads) {
-        int sum = 0;
-        for (int r = 0; r < kEvictCluster; ++r) sum += cluster.map_shared_rank(hist, r)[i];
-        total[i] = sum;
-      }
-      __syncthreads();
-      if (warp == 0) {
-        // Digits from the largest down, eight to a lane.
-        constexpr int kPer = kDigits / 32;
-        int mine = 0;
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) mine += total[kDigits - 1 - (lane * kPer + j)];
-        int incl = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int x = __shfl_up_sync(0xffffffffu, incl, o);
-          if (lane >= o) incl += x;
-        }
-        int before = incl - mine;
-        if (before < need && need <= incl) {
-          for (int j = 0; j < kPer; ++j) {
-            const int digit = kDigits - 1 - (lane * kPer + j);
-            if (before + total[digit] >= need) {
-              pick[0] = digit;
-              pick[1] = need - before;
-              break;
-            }
-            before += total[digit];
-          }
-        }
-      }
-      __syncthreads();
-      prefix |= static_cast<uint32_t>(pick[0]) << shift;
-      need = pick[1];
-      cluster.sync();  // every CTA has read the counts before they are cleared
-    }
-  }
-  // Now keys above `prefix` are kept, and the first `need` that equal it.
-
-  int n_above = 0, n_at = 0;
-  for (int t = t0 + tid; t < t1; t += kEvictThreads) {
-    const bool in = t >= lo && t < hi;
-    const uint32_t key = in ? weight_key(win[t]) : 0u;
-    n_above += !in || (need > 0 && key > prefix);
-    n_at += in && need > 0 && key == prefix;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    n_above += __shfl_xor_sync(0xffffffffu, n_above, o);
-    n_at += __shfl_xor_sync(0xffffffffu, n_at, o);
-  }
-  if (lane == 0) {
-    warp_sum[0][warp] = n_above;
-    warp_sum[1][warp] = n_at;
-  }
-  __syncthreads();
-  if (tid == 0) {
-    int a = 0, c = 0;
-    for (int i = 0; i < kEvictThreads / 32; ++i) {
-      a += warp_sum[0][i];
-      c += warp_sum[1][i];
-    }
-    above_of[0] = a;
-    above_of[1] = c;
-  }
-  cluster.sync();
-  int base_above = 0, base_at = 0;
-  for (int r = 0; r < rank; ++r) {
-    base_above += cluster.map_shared_rank(above_of, r)[0];
-    base_at += cluster.map_shared_rank(above_of, r)[1];
-  }
-  // Ranks within the slice: running counts of kept-for-sure and of ties.
-  for (int c0 = t0; c0 < t1; c0 += kEvictThreads) {
-    const int t = c0 + tid;
-    const bool in = t >= lo && t < hi;
-    const uint32_t key = (t < t1 && in) ? weight_key(win[t]) : 0u;
-    const bool sure = t < t1 && (!in || (need > 0 && key > prefix));
-    const bool tie = t < t1 && in && need > 0 && key == prefix;
-    const uint32_t bs = __ballot_sync(0xffffffffu, sure), bt = __ballot_sync(0xffffffffu, tie);
+  if (is_short) {
+    if (rank > 0) return;
+    // Thread i takes tokens [i * items, (i + 1) * items), through shared
+    // memory (one word of padding after 16) so that the loads are coalesced.
+    const int items = (len + kEvictThreads - 1) / kEvictThreads;
+    for (int t = tid; t < len; t += kEvictThreads) list[t + (t >> 4)] = __float_as_int(win[t]);
     __syncthreads();
+    int bits[kItems];
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      const int t = tid * items + i;
+      bits[i] = i < items && t < len ? list[t + (t >> 4)] : 0;
+    }
+    auto key_of = [&](int i) { return weight_key(__int_as_float(bits[i])); };
+    Selected sel{0xffffffffu, 0};
+    if (wanted > 0) {
+      uint32_t prefix = 0;
+      int need = wanted;
+      for (int shift = 32 - kDigitBits; shift >= 0; shift -= kDigitBits) {
+        for (int i = tid; i < kCopiesOfHist * kHistPitch; i += kEvictThreads) sh.hist[i] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kItems; ++i) {
+          const int t = tid * items + i;
+          if (i < items && t >= lo && t < hi) count_digit(sh, key_of(i), prefix, shift);
+        }
+        __syncthreads();
+        if (tid < kDigits) {
+          int sum = 0;
+#pragma unroll
+          for (int c = 0; c < kCopiesOfHist; ++c) sum += sh.hist[c * kHistPitch + tid];
+          sh.total[tid] = sum;
+        }
+        __syncthreads();
+        if (warp == 0) pick_digit(sh, need);
+        __syncthreads();
+        prefix |= static_cast<uint32_t>(sh.pick[0]) << shift;
+        need = sh.pick[1];
+        if (need == sh.pick[2]) {
+          // Every key of this digit is wanted: the ones from prefix up. (prefix
+          // is not 0: then all candidates would be kept.)
+          prefix -= 1;
+          need = 0;
+          break;
+        }
+      }
+      sel = Selected{prefix, need};
+    }
+    // Ranks: kept-for-sure tokens in the low half, ties in the high half.
+    uint32_t mine = 0;
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      const int t = tid * items + i;
+      if (i < items && t < len) {
+        const bool in = t >= lo && t < hi;
+        mine += (!in || (wanted > 0 && key_of(i) > sel.bound)) ? 1u : 0u;
+        mine += (in && sel.ties > 0 && key_of(i) == sel.bound) ? 0x10000u : 0u;
+      }
+    }
+    uint32_t incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t x = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += x;
+    }
+    if (lane == 31) sh.warp_sum[0][warp] = static_cast<int>(incl);
+    __syncthreads();  // also: every weight is in registers, list may be overwritten
+    uint32_t at = incl - mine;
+#pragma unroll
+    for (int i = 0; i < kEvictWarps; ++i) at += i < warp ? static_cast<uint32_t>(sh.warp_sum[0][i]) : 0u;
+    int sure = static_cast<int>(at & 0xffffu), tied = static_cast<int>(at >> 16);
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      const int t = tid * items + i;
+      if (i < items && t < len) {
+        const bool in = t >= lo && t < hi;
+        const bool yes = !in || (wanted > 0 && key_of(i) > sel.bound);
+        const bool tie = in && sel.ties > 0 && key_of(i) == sel.bound;
+        // Kept before this token: the sure ones and the ties among the first `ties`.
+        if (yes || (tie && tied < sel.ties)) {
+          const int j = sure + (tied < sel.ties ? tied : sel.ties);
+          list[j] = t;
+          kept_bits[j] = bits[i];
+        }
+        sure += yes;
+        tied += tie;
+      }
+    }
+    __syncthreads();
+    for (int j = tid; j < p.budget; j += kEvictThreads) kept[j] = j < keep ? list[j] : -1;
+    for (int j = tid; j < len; j += kEvictThreads) wout[j] = j < keep ? __int_as_float(kept_bits[j]) : 0.f;
+  } else {
+    // Counted together: every CTA takes a slice.
+    const int per = (len + ctas - 1) / ctas;
+    const int t0 = min(len, rank * per), t1 = min(len, t0 + per);
+    uint32_t prefix = 0xffffffffu;
+    int need = wanted;
+    if (need > 0) {
+      prefix = 0;
+      for (int shift = 32 - kDigitBits; shift >= 0; shift -= kDigitBits) {
+        for (int i = tid; i < kCopiesOfHist * kHistPitch; i += kEvictThreads) sh.hist[i] = 0;
+        __syncthreads();
+        for (int t = max(t0, lo) + tid; t < min(t1, hi); t += kEvictThreads) count_digit(sh, weight_key(win[t]), prefix, shift);
+        __syncthreads();
+        if (tid < kDigits) {
+          int sum = 0;
+#pragma unroll
+          for (int c = 0; c < kCopiesOfHist; ++c) sum += sh.hist[c * kHistPitch + tid];
+          sh.hist[tid] = sum;  // the first copy: only this thread reads and writes column tid
+        }
+        sync_cluster();
+        if (tid < kDigits) {
+          int sum = 0;
+          for (int r = 0; r < ctas; ++r) sum += ctas > 1 ? cluster.map_shared_rank(sh.hist, r)[tid] : sh.hist[tid];
+          sh.total[tid] = sum;
+        }
+        __syncthreads();
+        if (warp == 0) pick_digit(sh, need);
+        sync_cluster();  // pick is there, and every CTA has read the counts
+        prefix |= static_cast<uint32_t>(sh.pick[0]) << shift;
+        need = sh.pick[1];
+        if (need == sh.pick[2]) {
+          prefix -= 1;
+          need = 0;
+          break;
+        }
+      }
+    }
+    const bool some = wanted > 0;
+    int n_sure = 0, n_tie = 0;
+    for (int t = t0 + tid; t < t1; t += kEvictThreads) {
+      const bool in = t >= lo && t < hi;
+      const uint32_t key = in ? weight_key(win[t]) : 0u;
+      n_sure += !in || (some && key > prefix);
+      n_tie += in && need > 0 && key == prefix;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      n_sure += __shfl_xor_sync(0xffffffffu, n_sure, o);
+      n_tie += __shfl_xor_sync(0xffffffffu, n_tie, o);
+    }
     if (lane == 0) {
-      warp_sum[0][warp] = __popc(bs);
-      warp_sum[1][warp] = __popc(bt);
+      sh.warp_sum[0][warp] = n_sure;
+      sh.warp_sum[1][warp] = n_tie;
     }
     __syncthreads();
-    int a = base_above, c = base_at;
-    for (int i = 0; i < kEvictThreads / 32; ++i) {
-      if (i < warp) {
-        a += warp_sum[0][i];
-        c += warp_sum[1][i];
+    if (tid == 0) {
+      int a = 0, c = 0;
+      for (int i = 0; i < kEvictWarps; ++i) {
+        a += sh.warp_sum[0][i];
+        c += sh.warp_sum[1][i];
       }
-      base_above += warp_sum[0][i];
-      base_at += warp_sum[1][i];
+      sh.slice[0] = a;
+      sh.slice[1] = c;
     }
-    const uint32_t below = (1u << lane) - 1u;
-    a += __popc(bs & below);
-    c += __popc(bt & below);
-    // Kept before this token: the sure ones and the ties among the first `need`.
-    if (sure || (tie && c < need)) kept[a + (c < need ? c : need)] = t;
-  }
-  for (int j = keep + rank * kEvictThreads + tid; j < p.budget; j += kEvictCluster * kEvictThreads) kept[j] = -1;
-  if (h == 0 && rank == 0 && tid == 0) p.new_lens[b] = keep;
-  __threadfence();
-  cluster.sync();
-
-  // Move rows and weights, a step of kStep kept tokens at a time.
-  const int pieces = p.D / 8;                              // 16-byte pieces per row
-  const int rows_cta = kEvictThreads * kMoveRows / pieces;  // kept tokens per CTA and step
-  const int step = rows_cta * kEvictCluster;
-  for (int j0 = 0; j0 < keep; j0 += step) {
-    uint4 kx[kMoveRows], vx[kMoveRows];
-    int64_t kd[kMoveRows], vd[kMoveRows];
+    sync_cluster();
+    int base_sure = 0, base_tie = 0;
+    for (int r = 0; r < rank; ++r) {
+      base_sure += cluster.map_shared_rank(sh.slice, r)[0];
+      base_tie += cluster.map_shared_rank(sh.slice, r)[1];
+    }
+    for (int c0 = t0; c0 < t1; c0 += kEvictThreads) {
+      const int t = c0 + tid;
+      const bool in = t >= lo && t < hi;
+      const uint32_t key = (t < t1 && in) ? weight_key(win[t]) : 0u;
+      const bool sure = t < t1 && (!in || (some && key > prefix));
+      const bool tie = t < t1 && in && need > 0 && key == prefix;
+      const uint32_t bs = __ballot_sync(0xffffffffu, sure), bt = __ballot_sync(0xffffffffu, tie);
+      __syncthreads();
+      if (lane == 0) {
+        sh.warp_sum[0][warp] = __popc(bs);
+        sh.warp_sum[1][warp] = __popc(bt);
+      }
+      __syncthreads();
+      int a = base_sure, c = base_tie;
 #pragma unroll
-    for (int i = 0; i < kMoveRows; ++i) {
-      const int r = (tid + i * kEvictThreads) / pieces, piece = (tid + i * kEvictThreads) % pieces;
-      const int j = j0 + rank * rows_cta + r;
-      kd[i] = -1;
-      if (r < rows_cta && j < keep && j < p.out_capacity) {
-        const int src = kept[j];
-        const int sb = static_cast<int>(page_of(p.page, src)), db = static_cast<int>(page_of(p.page, j));
-        const int sp = p.tables[b * p.table_stride + sb], dp = p.out_tables[b * p.out_stride + db];
-        if (sp >= 0 && sp < p.num_pages && dp >= 0 && dp < p.num_pages) {
-          const int64_t srow = src - static_cast<int64_t>(sb) * p.page.size, drow = j - static_cast<int64_t>(db) * p.page.size;
-          const uint16_t* ks = static_cast<const uint16_t*>(p.k.base) + sp * p.k.page_stride + h * p.k.head_stride +
-                               srow * p.k.token_stride + piece * 8;
-          const uint16_t* vs = static_cast<const uint16_t*>(p.v.base) + sp * p.v.page_stride + h * p.v.head_stride +
-                               srow * p.v.token_stride + piece * 8;
-          if (!(sp == dp && srow == drow)) {
-            kx[i] = *reinterpret_cast<const uint4*>(ks);
-            vx[i] = *reinterpret_cast<const uint4*>(vs);
-            kd[i] = dp * p.k.page_stride + h * p.k.head_stride + drow * p.k.token_stride + piece * 8;
-            vd[i] = dp * p.v.page_stride + h * p.v.head_stride + drow * p.v.token_stride + piece * 8;
-          }
+      for (int i = 0; i < kEvictWarps; ++i) {
+        if (i < warp) {
+          a += sh.warp_sum[0][i];
+          c += sh.warp_sum[1][i];
+        }
+        base_sure += sh.warp_sum[0][i];
+        base_tie += sh.warp_sum[1][i];
+      }
+      const uint32_t below = (1u << lane) - 1u;
+      a += __popc(bs & below);
+      c += __popc(bt & below);
+      if (sure || (tie && c < need)) kept[a + (c < need ? c : need)] = t;
+    }
+    for (int j = keep + rank * kEvictThreads + tid; j < p.budget; j += ctas * kEvictThreads) kept[j] = -1;
+    __threadfence();
+    sync_cluster();  // the list is there for all
+    // The weights move a step at a time, as the rows below.
+    for (int j0 = 0; j0 < len; j0 += ctas * kEvictThreads) {
+      const int j = j0 + rank * kEvictThreads + tid;
+      const float x = j < keep ? win[kept[j]] : 0.f;
+      sync_cluster();
+      if (j < len) wout[j] = x;
+    }
+  }
+  if (h == 0 && rank == 0 && tid == 0) p.new_lens[b] = keep;
+
+}
+
+// The length of a sequence as the select kernel sees it, and what it keeps.
+__device__ __forceinline__ int kept_tokens(const EvictParams& p, int b) {
+  int len = p.lens[b];
+  len = len < 0 ? 0 : (len > p.capacity ? p.capacity : len);
+  return len < p.budget ? len : p.budget;
+}
+
+// Where token `t` of sequence b lies: page (negative: nowhere) and row.
+__device__ __forceinline__ int2 place_of(const EvictParams& p, const int32_t* table, int t) {
+  const int block = static_cast<int>(page_of(p.page, t));
+  const int page = table[block];
+  return make_int2(page < p.num_pages ? page : -1, t - block * static_cast<int>(p.page.size));
+}
+
+// Apart: a warp takes kApartRows kept tokens; each half of it looks up one end
+// of the moves, a token to a lane, so that the chain index -> table -> row is
+// walked once for all of them, and the rows then pass through registers with
+// kApartLoads vectors per lane in flight.
+constexpr int kApartWarps = 8;
+constexpr int kApartRows = 16;
+constexpr int kApartLoads = 4;
+
+__global__ void __launch_bounds__(kApartWarps * 32) kv_move_apart_kernel(const __grid_constant__ EvictParams p) {
+  const int seg = blockIdx.x;
+  const int b = seg / p.hkv, h = seg % p.hkv;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int keep = min(kept_tokens(p, b), p.out_capacity);
+  const int32_t* kept = p.kept + (static_cast<int64_t>(b) * p.hkv + h) * p.budget;
+  const int pieces = p.D / 8, row_items = 2 * pieces;
+  pdl_wait();
+  pdl_launch_dependents();
+  for (int j0 = (blockIdx.y * kApartWarps + warp) * kApartRows; j0 < keep; j0 += gridDim.y * kApartWarps * kApartRows) {
+    const int mine = j0 + (lane & (kApartRows - 1));
+    int2 place = make_int2(-1, 0);
+    if (mine < keep) {
+      place = lane < kApartRows ? place_of(p, p.tables + b * p.table_stride, kept[mine])
+                                : place_of(p, p.out_tables + b * p.out_stride, mine);
+    }
+    const int items = min(kApartRows, keep - j0) * row_items;
+    for (int i0 = 0; i0 < items; i0 += 32 * kApartLoads) {
+      uint4 x[kApartLoads];
+      uint16_t* dst[kApartLoads];
+#pragma unroll
+      for (int i = 0; i < kApartLoads; ++i) {
+        const int item = i0 + i * 32 + lane;
+        const int r = min(p.row_shift >= 0 ? item >> p.row_shift : item / row_items, kApartRows - 1);
+        const int sp = __shfl_sync(0xffffffffu, place.x, r), sr = __shfl_sync(0xffffffffu, place.y, r);
+        const int dp = __shfl_sync(0xffffffffu, place.x, kApartRows + r);
+        const int dr = __shfl_sync(0xffffffffu, place.y, kApartRows + r);
+        dst[i] = nullptr;
+        if (item < items && sp >= 0 && dp >= 0) {
+          const int at = item - r * row_items;
+          const PagedCache& cache = at < pieces ? p.k : p.v;
+          uint16_t* head = static_cast<uint16_t*>(cache.base) + h * cache.head_stride + (at < pieces ? at : at - pieces) * 8;
+          x[i] = *reinterpret_cast<const uint4*>(head + sp * cache.page_stride + sr * cache.token_stride);
+          dst[i] = head + dp * cache.page_stride + dr * cache.token_stride;
         }
       }
-    }
-    cluster.sync();  // the step's rows are in registers everywhere
 #pragma unroll
-    for (int i = 0; i < kMoveRows; ++i) {
-      if (kd[i] >= 0) {
-        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.k.base) + kd[i]) = kx[i];
-        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.v.base) + vd[i]) = vx[i];
+      for (int i = 0; i < kApartLoads; ++i) {
+        if (dst[i] != nullptr) *reinterpret_cast<uint4*>(dst[i]) = x[i];
       }
     }
   }
-  // The weights move the same way, one token per thread.
-  for (int j0 = 0; j0 < len; j0 += kEvictCluster * kEvictThreads) {
-    const int j = j0 + rank * kEvictThreads + tid;
-    const float x = j < keep ? win[kept[j]] : 0.f;
-    cluster.sync();
-    if (j < len) wout[j] = x;
+}
+
+// In place: a cluster per (sequence, kv head).
+__global__ void __launch_bounds__(kMoveThreads) kv_move_in_place_kernel(const __grid_constant__ EvictParams p) {
+  extern __shared__ __align__(16) unsigned char move_ring[];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ctas = static_cast<int>(cluster.num_blocks());
+  const int rank = static_cast<int>(cluster.block_rank());
+  const int seg = blockIdx.x / ctas;
+  const int b = seg / p.hkv, h = seg % p.hkv;
+  const int tid = threadIdx.x;
+  const int keep = kept_tokens(p, b);
+  const int32_t* kept = p.kept + (static_cast<int64_t>(b) * p.hkv + h) * p.budget;
+  pdl_wait();
+  pdl_launch_dependents();
+  // The rows move through a ring in shared memory that cp.async fills; a thread
+  // moves one piece of one row per step and cache, and reads only what it
+  // copied itself.
+  const int pieces = p.D / 8;                 // 16-byte pieces per row
+  const int rows_cta = kMoveThreads / pieces;  // kept tokens per CTA and step
+  const int step = rows_cta * ctas;
+  const int row = tid / pieces, piece = tid - row * pieces;
+  const int steps = (keep + step - 1) / step;
+  const uint32_t ring = smem_u32(move_ring) + tid * 16;
+  uint32_t live = 0;  // bit k: the newest step but k moves this thread's piece
+  auto fetch = [&](int k) {
+    const int j = k * step + rank * rows_cta + row;
+    bool moves = k < steps && row < rows_cta && j < keep && j < p.out_capacity;
+    if (moves) {
+      const int src = kept[j];
+      const int sb = static_cast<int>(page_of(p.page, src)), db = static_cast<int>(page_of(p.page, j));
+      const int sp = p.tables[b * p.table_stride + sb], dp = p.out_tables[b * p.out_stride + db];
+      const int srow = src - sb * static_cast<int>(p.page.size), drow = j - db * static_cast<int>(p.page.size);
+      moves = sp >= 0 && sp < p.num_pages && dp >= 0 && dp < p.num_pages && !(sp == dp && srow == drow);
+      if (moves) {
+        const uint32_t dst = ring + (k % kMoveStages) * (2 * kMoveThreads * 16);
+        cp_async16(dst, static_cast<const uint16_t*>(p.k.base) + sp * p.k.page_stride + h * p.k.head_stride +
+                            srow * p.k.token_stride + piece * 8);
+        cp_async16(dst + kMoveThreads * 16, static_cast<const uint16_t*>(p.v.base) + sp * p.v.page_stride +
+                                                 h * p.v.head_stride + srow * p.v.token_stride + piece * 8);
+      }
+    }
+    cp_async_commit();
+    live = (live << 1) | (moves ? 1u : 0u);
+  };
+#pragma unroll
+  for (int k = 0; k < kMoveStages - 1; ++k) fetch(k);
+  for (int k = 0; k < steps; ++k) {
+    // This thread's piece of step k has landed, then everybody's: from here on
+    // the rows that step k overwrites are read by nobody.
+    cp_async_wait<kMoveStages - 2>();
+    if (ctas > 1) {
+      cluster_barrier_relaxed();
+    } else {
+      __syncthreads();
+    }
+    if ((live >> (kMoveStages - 2)) & 1) {
+      const int j = k * step + rank * rows_cta + row;
+      const int db = static_cast<int>(page_of(p.page, j));
+      const int dp = p.out_tables[b * p.out_stride + db];
+      const int drow = j - db * static_cast<int>(p.page.size);
+      const unsigned char* at = move_ring + tid * 16 + (k % kMoveStages) * (2 * kMoveThreads * 16);
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.k.base) + dp * p.k.page_stride + h * p.k.head_stride +
+                                drow * p.k.token_stride + piece * 8) = *reinterpret_cast<const uint4*>(at);
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.v.base) + dp * p.v.page_stride + h * p.v.head_stride +
+                                drow * p.v.token_stride + piece * 8) =
+          *reinterpret_cast<const uint4*>(at + kMoveThreads * 16);
+    }
+    fetch(k + kMoveStages - 1);
   }
 }
 
@@ -389,8 +705,9 @@ int neso_rope_paged_append(const void* q, const void* k, const void* v, const fl
   if (page_size < 1) return fail(NESO_ERR_INVALID_ARG, "page_size must be at least 1 (got %d)", page_size);
   if (axes < 1 || axes > kMaxAxes) return fail(NESO_ERR_INVALID_ARG, "axes must be in [1, %d] (got %d)", kMaxAxes, axes);
   if (axes > 1 && sections == nullptr) return fail(NESO_ERR_INVALID_ARG, "several axes need their sections");
-  if (static_cast<int64_t>(Hq + static_cast<int64_t>(Hkv) * 2) * D > INT32_MAX) {
-    return fail(NESO_ERR_UNSUPPORTED, "a token has more than 2^31 - 1 elements");
+  if (D > kMaxRopeDim) return fail(NESO_ERR_UNSUPPORTED, "head_dim is limited to %d (got %d)", kMaxRopeDim, D);
+  if (static_cast<int64_t>(Hq) + 2 * static_cast<int64_t>(Hkv) > 65536) {
+    return fail(NESO_ERR_UNSUPPORTED, "a token has more than 65536 heads");
   }
   RopeParams p{};
   int at = 0;
@@ -436,9 +753,10 @@ int neso_rope_paged_append(const void* q, const void* k, const void* v, const fl
   p.table_rows = table_rows;
   p.axes = axes;
   p.page = page_divisor(static_cast<uint32_t>(page_size));
+  p.heads = page_divisor(static_cast<uint32_t>(Hq + 2 * Hkv > 0 ? Hq + 2 * Hkv : 1));
   // 16-byte vectors where the rows of q, k, v and q_out start on them and the
-  // rotated part ends on one.
-  const bool vec = half % 8 == 0 && aligned16(q) && aligned16(k) && aligned16(v) && aligned16(q_out) &&
+  // rotated part and the rest are pairs of them.
+  const bool vec = D % 16 == 0 && half % 8 == 0 && aligned16(q) && aligned16(k) && aligned16(v) && aligned16(q_out) &&
                    (q_stride_n | q_stride_h | k_stride_n | k_stride_h | v_stride_n | v_stride_h) % 8 == 0;
   if (dtype == NESO_BF16) return vec ? launch_rope<true, 8>(p, as_stream(stream)) : launch_rope<true, 1>(p, as_stream(stream));
   return vec ? launch_rope<false, 8>(p, as_stream(stream)) : launch_rope<false, 1>(p, as_stream(stream));
@@ -462,7 +780,7 @@ int neso_kv_evict(void* k_cache, void* v_cache, const int32_t* block_tables, con
   if (budget < 1 || recent < 0 || sink < 0 || static_cast<int64_t>(recent) + sink > budget) {
     return fail(NESO_ERR_INVALID_ARG, "need budget >= 1 and 0 <= recent + sink <= budget");
   }
-  if (static_cast<int64_t>(B) * Hkv * kEvictCluster > INT32_MAX) {
+  if (static_cast<int64_t>(B) * Hkv * kMaxCluster > INT32_MAX) {
     return fail(NESO_ERR_UNSUPPORTED, "batch x heads is too large");
   }
   if (B == 0) return ok();
@@ -502,9 +820,51 @@ int neso_kv_evict(void* k_cache, void* v_cache, const int32_t* block_tables, con
   p.capacity = static_cast<int>(cap < (1 << 30) ? cap : (1 << 30));
   p.out_capacity = static_cast<int>(ocap < (1 << 30) ? ocap : (1 << 30));
   p.page = page_divisor(static_cast<uint32_t>(page_size));
-  cudaError_t e = launch_pdl(kv_evict_kernel, dim3(static_cast<unsigned>(B) * Hkv * kEvictCluster), dim3(kEvictThreads), 0,
-                             as_stream(stream), p);
-  return e == cudaSuccess ? ok() : cuda_fail(e, "kv_evict launch");
+  const int64_t segments = static_cast<int64_t>(B) * Hkv;
+  const int pieces = D / 8;
+  p.row_shift = -1;
+  for (int i = 0; i < 7; ++i) {
+    if ((1 << i) == 2 * pieces) p.row_shift = i;
+  }
+  auto launch = [&](void (*kern)(EvictParams), int ctas, int threads, int smem) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(segments * ctas));
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = as_stream(stream);
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(ctas);
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, kern, p);
+  };
+  // CTAs that count one long sequence: as many as the SMs hold two deep.
+  int ctas = 1;
+  while (cap > kShortLen && ctas < kMaxCluster && segments * ctas * 2 <= 2 * sm_count()) ctas *= 2;
+  int rc = kernel_setup(reinterpret_cast<const void*>(kv_select_kernel), kSelectBytes, nullptr);
+  if (rc != NESO_OK) return rc;
+  cudaError_t e = launch(kv_select_kernel, ctas, kEvictThreads, kSelectBytes);
+  if (e != cudaSuccess) return cuda_fail(e, "kv_evict select launch");
+  const int64_t most = budget < cap ? budget : cap;
+  if (out_tables != block_tables) {
+    const int64_t blocks = (most + kApartWarps * kApartRows - 1) / (kApartWarps * kApartRows);
+    if (blocks == 0) return ok();
+    e = launch_pdl(kv_move_apart_kernel, dim3(static_cast<unsigned>(segments), static_cast<unsigned>(blocks < 65535 ? blocks : 65535)),
+                   dim3(kApartWarps * 32), 0, as_stream(stream), p);
+  } else {
+    rc = kernel_setup(reinterpret_cast<const void*>(kv_move_in_place_kernel), kMoveBytes, nullptr);
+    if (rc != NESO_OK) return rc;
+    // As many as fill the SMs two deep, no more than have a step's rows to move.
+    const int rows = kMoveThreads / pieces;
+    for (ctas = 1; ctas < kMaxCluster && segments * ctas * 2 <= 2 * sm_count() && static_cast<int64_t>(rows) * ctas < most;) ctas *= 2;
+    e = launch(kv_move_in_place_kernel, ctas, kMoveThreads, kMoveBytes);
+  }
+  return e == cudaSuccess ? ok() : cuda_fail(e, "kv_evict move launch");
 }
 
 }  // extern "C"

@@ -491,6 +491,8 @@ def _check_evict(seed, dtype, lens, hkv, D, page, budget, recent, sink, mode, we
     ([333, 9], 3, 8, 24, 300, 100, 4),
     ([50], 1, 256, 16, 49, 0, 49),
     ([5000], 2, 64, 64, 4321, 17, 3),
+    ([8192, 8193, 300], 1, 64, 64, 5000, 17, 3),  # on both sides of the change to counting together
+    ([20000], 1, 8, 256, 12345, 1, 0),
 ])
 def test_evict(dev, lens, hkv, D, page, budget, recent, sink, mode):
     _check_evict(len(lens) + D, TYPES[D % 3 % 2], lens, hkv, D, page, budget, recent, sink, mode)

@@ -13,6 +13,7 @@ from pathlib import Path
 
 _PKG = Path(__file__).resolve().parent
 LIB_PATH = _PKG / "libneso_b200.so"
+BINDING_PATH = _PKG / "_bindings.so"
 HEADER_PATH = _PKG.parent / "include" / "neso_b200.h"
 
 NESO_OK = 0
@@ -137,6 +138,29 @@ def lib() -> ctypes.CDLL:
         fn.argtypes = args
     _lib = handle
     return handle
+
+
+def binding():
+    """Load the extension module behind the decoding-step operators of ``ops``
+    and hand it the library's entry points. Raises NesoLibraryError if absent."""
+    import importlib.machinery
+    import importlib.util
+
+    import torch  # noqa: F401  (the module links against the libraries that torch loads)
+
+    if not BINDING_PATH.exists():
+        raise NesoLibraryError(f"{BINDING_PATH} is missing: build it with `python -m neso_b200.build`")
+    loader = importlib.machinery.ExtensionFileLoader("_bindings", str(BINDING_PATH))
+    try:
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_bindings", loader))
+        loader.exec_module(module)
+    except ImportError as e:
+        raise NesoLibraryError(f"failed to load {BINDING_PATH}: {e}") from e
+    handle = lib()
+    names = ("neso_set_device", "neso_rope_paged_append", "neso_paged_attention", "neso_paged_attention_workspace",
+             "neso_kv_evict", "neso_process_logits")
+    module.set_entry_points(check, *(ctypes.cast(getattr(handle, n), ctypes.c_void_p).value for n in names))
+    return module
 
 
 def last_error() -> str:

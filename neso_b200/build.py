@@ -7,6 +7,11 @@ machine without a GPU driver (the driver is reached lazily through
 ``cudaGetDriverEntryPoint``). Objects are rebuilt only when a source or header
 is newer than them.
 
+``csrc/bindings.cpp``, the extension module behind the decoding-step operators
+of ``ops``, is compiled with g++ against torch's headers into
+``_bindings.so``; it reaches the kernels through the library that ``_lib``
+loads and links against torch alone.
+
 Usage: ``python -m neso_b200.build [--force] [-v] [--ptxas-info]``
 """
 from __future__ import annotations
@@ -24,6 +29,8 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 BUILD = ROOT / "_build"
 LIB = PKG / "libneso_b200.so"
+BINDING_SRC = CSRC / "bindings.cpp"
+BINDING = PKG / "_bindings.so"
 HARNESS_SRC = PKG / "harness" / "neso_harness.cpp"
 HARNESS = PKG / "neso_harness"
 
@@ -69,8 +76,10 @@ def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) 
     sources = sorted(CSRC.glob("*.cu"))
     if not sources:
         raise RuntimeError(f"no CUDA sources under {CSRC}")
-    with cf.ThreadPoolExecutor(max_workers=min(8, len(sources))) as ex:
+    with cf.ThreadPoolExecutor(max_workers=8) as ex:
+        binding = ex.submit(build_binding, force)
         results = list(ex.map(lambda s: _compile(s, force, ptxas_info), sources))
+        binding.result()
     objs = [o for o, _ in results]
     if verbose or ptxas_info:
         for o, log in results:
@@ -85,6 +94,30 @@ def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) 
         os.replace(tmp, LIB)
     build_harness(force)
     return LIB
+
+
+def build_binding(force: bool = False) -> Path:
+    """Compile the extension module against the installed torch."""
+    import sysconfig
+
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    newest = max(p.stat().st_mtime for p in (BINDING_SRC, root / "version.py", ROOT / "include" / "neso_b200.h"))
+    if not force and BINDING.exists() and BINDING.stat().st_mtime > newest:
+        return BINDING
+    cuda = Path(nvcc()).resolve().parent.parent
+    includes = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include",
+                sysconfig.get_paths()["include"], cuda / "include"]
+    tmp = BINDING.with_suffix(".so.tmp")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{i}" for i in includes),
+           str(BINDING_SRC), "-o", str(tmp), f"-L{root / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"building {BINDING.name} failed:\n{' '.join(cmd)}\n{res.stdout}\n{res.stderr}")
+    os.replace(tmp, BINDING)
+    return BINDING
 
 
 def build_harness(force: bool = False) -> Path:

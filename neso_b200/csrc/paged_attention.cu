@@ -20,7 +20,9 @@
 // cp.async (no block barrier), its own running maximum and sum. A run that
 // holds a whole (sequence, kv head) writes the output itself; a run's first
 // and last pieces leave their maximum, sum and unnormalised output in the
-// workspace, and a second kernel joins them.
+// workspace, and a second kernel joins them. Where the tables are short and
+// the (sequence, kv head) pairs fit the SMs, a CTA takes one pair and joins its
+// warps' parts itself: one launch, and no search for the runs.
 //
 // Products: the tokens are the M rows of mma.m16n8k16 and the query heads its
 // N columns (S^T = K Q^T, O^T = V^T P^T), so a group of up to 8 heads costs one
@@ -82,49 +84,37 @@ __device__ __forceinline__ Span span_of(const AttnParams& p, int b) {
 
 // The batch's work as a line: each segment, one (sequence, kv head, tile) with
 // visible tokens, is kStart points for starting it (its queries, its output)
-// followed by one point per unit. Runs are equal pieces of this line.
+// followed by one point per unit. Runs are equal pieces of this line, whose
+// length the host has checked to fit 31 bits.
 __device__ __forceinline__ int cost_of(const Span& s) { return s.u1 > s.u0 ? s.u1 - s.u0 + kStart : 0; }
 
 // Points per (kv head, tile) of the sequences before `b`, and of all of them;
 // a whole warp calls it.
-__device__ __forceinline__ void line_sums(const AttnParams& p, int b, int64_t* before, int64_t* all) {
-  const int lane = threadIdx.x & 31;
-  int64_t lo = 0, sum = 0;
-  for (int i = lane; i < p.B; i += 32) {
+__device__ __forceinline__ void line_sums(const AttnParams& p, int b, int* before, int* all) {
+  int lo = 0, sum = 0;
+  for (int i = threadIdx.x & 31; i < p.B; i += 32) {
     const int cost = cost_of(span_of(p, i));
     sum += cost;
     if (i < b) lo += cost;
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    lo += __shfl_xor_sync(0xffffffffu, lo, o);
-  }
-  *before = lo;
-  *all = sum;
-}
-
-// Quotient of non-negative values; nearly always both fit 32 bits, where the
-// division takes a fifth of the time.
-__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
-  if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
-  return a / b;
+  *all = __reduce_add_sync(0xffffffffu, sum);
+  *before = __reduce_add_sync(0xffffffffu, lo);
 }
 
 // The line of `total` points is cut into `count` runs; the first `longer` of
 // them have len + 1 points, the others len.
 struct Runs {
-  int64_t count, len, longer;
-  __device__ __forceinline__ Runs(const AttnParams& p, int64_t total) {
-    const int64_t most = total / kMinRun;
+  int count, len, longer;
+  __device__ __forceinline__ Runs(const AttnParams& p, int total) {
+    const int most = total / kMinRun;
     count = most < 1 ? 1 : (most < p.warps ? most : p.warps);
-    len = quotient(total, count);
+    len = total / count;
     longer = total - len * count;
   }
-  __device__ __forceinline__ int64_t begin(int64_t w) const { return w * len + (w < longer ? w : longer); }
-  __device__ __forceinline__ int64_t holding(int64_t x) const {
-    const int64_t bound = longer * (len + 1);
-    return x < bound ? quotient(x, len + 1) : longer + quotient(x - bound, len);
+  __device__ __forceinline__ int begin(int w) const { return w * len + (w < longer ? w : longer); }
+  __device__ __forceinline__ int holding(int x) const {
+    const int bound = longer * (len + 1);
+    return x < bound ? x / (len + 1) : longer + (x - bound) / len;
   }
 };
 
@@ -147,43 +137,56 @@ struct Cursor {
   }
 };
 
-// The first unit at or after point `at` of the line, and how many units come
-// before it; a whole warp calls it. Past the end of the line c.b is p.B.
-__device__ __forceinline__ Cursor find_unit(const AttnParams& p, int64_t at, int64_t* units_before) {
+// Run w: its first unit and how many units it has; a whole warp calls it.
+__device__ __forceinline__ int find_run(const AttnParams& p, int w, Cursor* first) {
   const int lane = threadIdx.x & 31;
   const int heads = p.hkv * p.tiles;
-  const int64_t point = at;
-  int64_t segments = 0;  // before the 32 sequences in hand
-  Cursor c{p.B, 0, 0, {0, 0, 0, 0}};
+  const int cost0 = lane < p.B ? cost_of(span_of(p, lane)) : 0;
+  int sum = cost0;
+  for (int i = lane + 32; i < p.B; i += 32) sum += cost_of(span_of(p, i));
+  const int total = __reduce_add_sync(0xffffffffu, sum) * heads;
+  const Runs runs(p, total);
+  if (total == 0 || w >= runs.count) return 0;
+  const int from = runs.begin(w), to = runs.begin(w + 1);
+  int units_from = 0, units_to = 0;
+  int past = 0, segments = 0;  // of the sequences before the 32 in hand
   for (int b0 = 0; b0 < p.B; b0 += 32) {
-    const int b = b0 + lane;
-    const int64_t mine = b < p.B ? static_cast<int64_t>(cost_of(span_of(p, b))) * heads : 0;
-    int64_t incl = mine;
+    const int cost = b0 == 0 ? cost0 : (b0 + lane < p.B ? cost_of(span_of(p, b0 + lane)) : 0);
+    int end = cost * heads;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t t = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += t;
+      const int t = __shfl_up_sync(0xffffffffu, end, o);
+      if (lane >= o) end += t;
     }
-    const uint32_t filled = __ballot_sync(0xffffffffu, mine > 0);
-    const uint32_t past = __ballot_sync(0xffffffffu, at < incl);
-    if (past != 0) {
-      const int src = __ffs(past) - 1;
-      const int64_t rest = at - __shfl_sync(0xffffffffu, incl - mine, src);
-      c.b = b0 + src;
-      c.s = span_of(p, c.b);
-      const int cost = cost_of(c.s);
-      c.hx = static_cast<int>(quotient(rest, cost));
-      const int in = static_cast<int>(rest - static_cast<int64_t>(c.hx) * cost);
-      c.u = c.s.u0 + (in > kStart ? in - kStart : 0);
-      segments += static_cast<int64_t>(__popc(filled & ((1u << src) - 1u))) * heads + c.hx;
-      *units_before = point - in - segments * kStart + (c.u - c.s.u0);
-      return c;
+    end += past;
+    const uint32_t filled = __ballot_sync(0xffffffffu, cost > 0);
+    const int all = __shfl_sync(0xffffffffu, end, 31);
+    // The first unit at or after point `at`, and the units before it.
+    auto locate = [&](int at, Cursor* c) {
+      const int src = __ffs(__ballot_sync(0xffffffffu, at < end)) - 1;
+      const int b_cost = __shfl_sync(0xffffffffu, cost, src);
+      const int start = __shfl_sync(0xffffffffu, end, src) - b_cost * heads;
+      const int hx = (at - start) / b_cost;
+      const int in = at - start - hx * b_cost;
+      const int unit = in > kStart ? in - kStart : 0;
+      const int seg = segments + __popc(filled & ((1u << src) - 1u)) * heads + hx;
+      if (c != nullptr) {
+        c->b = b0 + src;
+        c->s = span_of(p, c->b);
+        c->hx = hx;
+        c->u = c->s.u0 + unit;
+      }
+      return at - in + unit - seg * kStart;
+    };
+    if (from >= past && from < all) units_from = locate(from, first);
+    if (to >= past && to < all) {
+      units_to = locate(to, nullptr);
+      return units_to - units_from;
     }
-    segments += static_cast<int64_t>(__popc(filled)) * heads;
-    at -= __shfl_sync(0xffffffffu, incl, 31);
+    segments += __popc(filled) * heads;
+    past = all;
   }
-  *units_before = point - at - segments * kStart;
-  return c;
+  return total - segments * kStart - units_from;  // the last run ends with the line
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
@@ -265,52 +268,44 @@ __device__ __forceinline__ float safe_max(float m) { return m == -INFINITY ? 0.f
 // 1 / l, and 0 for a row that saw no token (l == 0); NaN stays NaN.
 __device__ __forceinline__ float inv_sum(float l) { return l == 0.f ? 0.f : __fdiv_rn(1.f, l); }
 
+// One warp's work: a ring of units, and the state of the segment in hand.
 // kBias: scores are capped or get a distance bias. kScores: they are kept for
-// the weights kernel.
+// the weights.
 template <bool kBf16, int D, int NT, bool kBias, bool kScores>
-__global__ void __launch_bounds__(kThreads, D == 128 ? 2 : 4)
-    paged_attention_kernel(const __grid_constant__ AttnParams p) {
-  constexpr int kRowBytes = D * 2;
-  constexpr int kHalf = kUnit * kRowBytes;  // K or V of one unit
-  constexpr int kChunks = kRowBytes / 16;   // 16-byte chunks per row
-  constexpr int kRowsPerCopy = 32 / kChunks;
-  constexpr int kCopies = kUnit / kRowsPerCopy;
-  extern __shared__ __align__(128) unsigned char smem[];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t ring = smem_u32(smem) + warp * (kStages * 2 * kHalf);
+struct Warp {
+  static constexpr int kRowBytes = D * 2;
+  static constexpr int kHalf = kUnit * kRowBytes;  // K or V of one unit
+  static constexpr int kRing = kStages * 2 * kHalf;
+  static constexpr int kChunks = kRowBytes / 16;   // 16-byte chunks per row
+  static constexpr int kRowsPerCopy = 32 / kChunks;
+  static constexpr int kCopies = kUnit / kRowsPerCopy;
 
-  // Released only here: the join kernel reads the lengths before its own wait,
-  // so everything launched before this grid has to be complete by then.
-  pdl_wait();
-  pdl_launch_dependents();
+  const AttnParams& p;
+  const int lane;
+  const uint32_t ring;
+  uint64_t masks;  // 16 validity bits per unit in flight, newest in the low bits
+  uint32_t qf[NT][D / 16][2];
+  float o[NT][D / 16][4];
+  float m[NT][2], l[NT][2], slope[NT][2];
+  int h0, nrows;
 
-  int64_t unused, per_head, units0, units1;
-  line_sums(p, 0, &unused, &per_head);
-  const int64_t total = per_head * p.hkv * p.tiles;
-  const Runs runs(p, total);
-  // Neighbouring runs go to different CTAs, so a small batch spreads over the SMs.
-  const int64_t w = static_cast<int64_t>(warp) * gridDim.x + blockIdx.x;
-  if (w >= runs.count) return;
-  Cursor ld = find_unit(p, runs.begin(w), &units0);
-  find_unit(p, runs.begin(w + 1), &units1);
-  const int n = static_cast<int>(units1 - units0);
-  if (n == 0) return;
-  Cursor c = ld;
-  uint64_t masks = 0;  // 16 validity bits per unit in flight, newest in the low bits
+  __device__ __forceinline__ Warp(const AttnParams& params, uint32_t ring_addr)
+      : p(params), lane(threadIdx.x & 31), ring(ring_addr), masks(0) {}
 
-  auto issue = [&](int stage, bool any) {
+  // Request unit c.u into a stage; with any = false only the group is counted.
+  __device__ __forceinline__ void request(const Cursor& c, int stage, bool any) {
     uint32_t valid_bits = 0;
     if (any) {
       const int chunk = lane % kChunks;
       const uint32_t base = ring + stage * (2 * kHalf);
-      const int64_t head = ld.hx / p.tiles;
-      const int t0 = ld.u * kUnit;
+      const int64_t head = c.hx / p.tiles;
+      const int t0 = c.u * kUnit;
       if (p.whole_units) {
         // A unit lies in one page: one table entry, rows a constant stride apart.
         const uint32_t block = page_of(p.page, t0);
-        const int page = p.tables[ld.b * p.table_stride + block];
+        const int page = p.tables[c.b * p.table_stride + block];
         if (page >= 0 && page < p.num_pages) {
-          const int a = ld.s.lo - t0, z = ld.s.len - t0;  // rows [a, z) are visible
+          const int a = c.s.lo - t0, z = c.s.len - t0;  // rows [a, z) are visible
           valid_bits = (z >= 16 ? 0xffffu : (1u << z) - 1u) & (a > 0 ? ~0u << a : ~0u);
         }
         const int64_t at = t0 - static_cast<int64_t>(block) * p.page.size + lane / kChunks;
@@ -332,12 +327,12 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? 2 : 4)
         // Lane r < 16 finds the address of key row r of the unit, lane 16 + r
         // that of value row r; the copies fetch them by shuffle.
         const int t = t0 + (lane & 15);
-        bool valid = t >= ld.s.lo && t < ld.s.len;
+        bool valid = t >= c.s.lo && t < c.s.len;
         const PagedCache& cache = lane < 16 ? p.k : p.v;
         int64_t off = 0;
         if (valid) {
           const uint32_t block = page_of(p.page, t);
-          const int page = p.tables[ld.b * p.table_stride + block];
+          const int page = p.tables[c.b * p.table_stride + block];
           valid = page >= 0 && page < p.num_pages;
           if (valid) {
             off = page * cache.page_stride + head * cache.head_stride +
@@ -358,59 +353,41 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? 2 : 4)
           }
         }
       }
-      ld.next(p);
     }
     masks = (masks << 16) | valid_bits;
     cp_async_commit();
-  };
+  }
 
+  // A new segment: its queries as the B operand (a head per lane quad), empty
+  // statistics.
+  __device__ __forceinline__ void start(const Cursor& c) {
+    const int tile = c.hx % p.tiles;
+    h0 = (c.hx / p.tiles) * p.group + tile * p.rows;
+    nrows = p.group - tile * p.rows < p.rows ? p.group - tile * p.rows : p.rows;
 #pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) issue(s, s < n);
-
-  uint32_t qf[NT][D / 16][2];
-  float o[NT][D / 16][4];
-  float m[NT][2], l[NT][2], slope[NT][2];
-  bool fresh = true, whole = false, first_piece = true;
-  int nrows = 0;
-
-  for (int i = 0, stage = 0; i < n; ++i) {
-    if (fresh) {
-      // A new (sequence, kv head, tile): its queries as the B operand (one
-      // head per lane quad row), empty statistics.
-      fresh = false;
-      whole = c.u == c.s.u0;
-      const int tile = c.hx % p.tiles;
-      const int h0 = (c.hx / p.tiles) * p.group + tile * p.rows;
-      nrows = p.group - tile * p.rows < p.rows ? p.group - tile * p.rows : p.rows;
+    for (int nt = 0; nt < NT; ++nt) {
+      const int row = nt * 8 + (lane >> 2);
+      const uint16_t* qrow = p.q + c.b * p.q_sb + static_cast<int64_t>(h0 + row) * p.q_sh + (lane & 3) * 2;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const int row = nt * 8 + (lane >> 2);
-        const uint16_t* qrow = p.q + c.b * p.q_sb + static_cast<int64_t>(h0 + row) * p.q_sh + (lane & 3) * 2;
+      for (int ks = 0; ks < D / 16; ++ks) {
+        qf[nt][ks][0] = row < nrows ? *reinterpret_cast<const uint32_t*>(qrow + ks * 16) : 0u;
+        qf[nt][ks][1] = row < nrows ? *reinterpret_cast<const uint32_t*>(qrow + ks * 16 + 8) : 0u;
+        o[nt][ks][0] = o[nt][ks][1] = o[nt][ks][2] = o[nt][ks][3] = 0.f;
+      }
 #pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) {
-          qf[nt][ks][0] = row < nrows ? *reinterpret_cast<const uint32_t*>(qrow + ks * 16) : 0u;
-          qf[nt][ks][1] = row < nrows ? *reinterpret_cast<const uint32_t*>(qrow + ks * 16 + 8) : 0u;
-          o[nt][ks][0] = o[nt][ks][1] = o[nt][ks][2] = o[nt][ks][3] = 0.f;
-        }
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          m[nt][j] = -INFINITY;
-          l[nt][j] = 0.f;
-          const int col = nt * 8 + (lane & 3) * 2 + j;
-          slope[nt][j] = (kBias && p.slopes != nullptr && col < nrows) ? p.slopes[h0 + col] * kLog2e : 0.f;
-        }
+      for (int j = 0; j < 2; ++j) {
+        m[nt][j] = -INFINITY;
+        l[nt][j] = 0.f;
+        const int col = nt * 8 + (lane & 3) * 2 + j;
+        slope[nt][j] = (kBias && p.slopes != nullptr && col < nrows) ? p.slopes[h0 + col] * kLog2e : 0.f;
       }
     }
+  }
 
-    cp_async_wait<kStages - 2>();
-    __syncwarp();
-    {
-      const int next = stage + kStages - 1;
-      issue(next >= kStages ? next - kStages : next, i + kStages - 1 < n);
-    }
+  // Add the unit that lies in a stage, the oldest requested.
+  __device__ __forceinline__ void add(const Cursor& c, int stage) {
     const uint32_t valid_bits = static_cast<uint32_t>(masks >> (16 * (kStages - 1))) & 0xffffu;
     const uint32_t base = ring + stage * (2 * kHalf);
-
     // S^T = K Q^T: rows are tokens lane/4 and lane/4 + 8, columns heads.
     float s[NT][4];
 #pragma unroll
@@ -432,21 +409,17 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? 2 : 4)
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        float x;
+        float x = s[nt][j] * p.score_scale;
         if (kBias) {
-          x = s[nt][j] * p.score_scale;
           if (p.softcap > 0.f) x = p.softcap * kLog2e * tanhf(x);
           const int t = c.u * kUnit + (lane >> 2) + (j >> 1) * 8;
           x = fmaf(slope[nt][j & 1], static_cast<float>(t - (c.s.len - 1)), x);
-        } else {
-          x = s[nt][j] * p.score_scale;
         }
         s[nt][j] = ((j >> 1) ? v1 : v0) ? x : -INFINITY;
       }
       if (kScores) {
         const int t = c.u * kUnit + (lane >> 2);
         const int col = nt * 8 + (lane & 3) * 2;
-        const int h0 = (c.hx / p.tiles) * p.group + (c.hx % p.tiles) * p.rows;
         float* dst = p.scores + (static_cast<int64_t>(c.b) * p.hq + h0 + col) * p.score_stride + t;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -502,40 +475,92 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? 2 : 4)
         }
       }
     }
+  }
+
+  // The sums of the segment's weights, over the lanes.
+  __device__ __forceinline__ void close() {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], d);
+      }
+    }
+  }
+  __device__ __forceinline__ float4 fragment(int nt, int dt) const {
+    return make_float4(o[nt][dt][0], o[nt][dt][1], o[nt][dt][2], o[nt][dt][3]);
+  }
+  __device__ __forceinline__ float4 stats(int nt) const { return make_float4(m[nt][0], l[nt][0], m[nt][1], l[nt][1]); }
+};
+
+template <bool kBf16, int D, int NT, bool kBias, bool kScores>
+__global__ void __launch_bounds__(kThreads, D == 128 ? 2 : 4)
+    paged_attention_kernel(const __grid_constant__ AttnParams p) {
+  using W = Warp<kBf16, D, NT, kBias, kScores>;
+  extern __shared__ __align__(128) unsigned char smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  // Released only here: the join kernel reads the lengths before its own wait,
+  // so everything launched before this grid has to be complete by then.
+  pdl_wait();
+  pdl_launch_dependents();
+
+  // Neighbouring runs go to different CTAs, so a small batch spreads over the SMs.
+  const int w = warp * gridDim.x + blockIdx.x;
+  Cursor ld;
+  const int n = find_run(p, w, &ld);
+  if (n == 0) return;
+  Cursor c = ld;
+  W my(p, smem_u32(smem) + warp * W::kRing);
+  auto request = [&](int stage, bool any) {
+    my.request(ld, stage, any);
+    if (any) ld.next(p);
+  };
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s) request(s, s < n);
+
+  bool fresh = true, whole = false, first_piece = true;
+  for (int i = 0, stage = 0; i < n; ++i) {
+    if (fresh) {
+      fresh = false;
+      whole = c.u == c.s.u0;
+      my.start(c);
+    }
+    cp_async_wait<kStages - 2>();
+    __syncwarp();
+    {
+      const int next = stage + kStages - 1;
+      request(next >= kStages ? next - kStages : next, i + kStages - 1 < n);
+    }
+    my.add(c, stage);
 
     const bool seg_end = c.u + 1 == c.s.u1;
     if (seg_end || i + 1 == n) {
-      const int h0 = (c.hx / p.tiles) * p.group + (c.hx % p.tiles) * p.rows;
+      my.close();
+      const int64_t head = static_cast<int64_t>(c.b) * p.hq + my.h0;
+      const int64_t slot = w * 2 + (first_piece ? 0 : 1);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-#pragma unroll
-          for (int d = 4; d < 32; d <<= 1) l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], d);
-        }
         if (whole && seg_end) {
-          const float r0 = inv_sum(l[nt][0]), r1 = inv_sum(l[nt][1]);
-          uint16_t* head0 = p.out + (static_cast<int64_t>(c.b) * p.hq + h0) * D;
+          const float r0 = inv_sum(my.l[nt][0]), r1 = inv_sum(my.l[nt][1]);
 #pragma unroll
           for (int dt = 0; dt < D / 16; ++dt) {
-            const float t[4] = {o[nt][dt][0] * r0, o[nt][dt][1] * r1, o[nt][dt][2] * r0, o[nt][dt][3] * r1};
-            store_out_tile<kBf16>(p, t, head0, D, nt, dt, nrows);
+            const float4 f = my.fragment(nt, dt);
+            const float t[4] = {f.x * r0, f.y * r1, f.z * r0, f.w * r1};
+            store_out_tile<kBf16>(p, t, p.out + head * D, D, nt, dt, my.nrows);
           }
           if (kScores && lane < 4) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
               const int col = nt * 8 + lane * 2 + j;
-              if (col < nrows) p.head_stats[static_cast<int64_t>(c.b) * p.hq + h0 + col] = make_float2(m[nt][j], l[nt][j]);
+              if (col < my.nrows) p.head_stats[head + col] = make_float2(my.m[nt][j], my.l[nt][j]);
             }
           }
         } else {
-          const int64_t slot = w * 2 + (first_piece ? 0 : 1);
 #pragma unroll
-          for (int dt = 0; dt < D / 16; ++dt) {
-            p.partials[((slot * NT + nt) * (D / 16) + dt) * 32 + lane] =
-                make_float4(o[nt][dt][0], o[nt][dt][1], o[nt][dt][2], o[nt][dt][3]);
-          }
-          if (lane < 4) p.stats[(slot * NT + nt) * 4 + lane] = make_float4(m[nt][0], l[nt][0], m[nt][1], l[nt][1]);
+          for (int dt = 0; dt < D / 16; ++dt) p.partials[((slot * NT + nt) * (D / 16) + dt) * 32 + lane] = my.fragment(nt, dt);
+          if (lane < 4) p.stats[(slot * NT + nt) * 4 + lane] = my.stats(nt);
         }
       }
       fresh = true;
@@ -546,22 +571,122 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? 2 : 4)
   }
 }
 
+// One CTA per (sequence, kv head) of one tile, its units dealt to the warps in turn;
+// the warps' parts are joined in shared memory, in a fixed order.
+constexpr int kSegWarps = 8;
+constexpr int kSegThreads = kSegWarps * 32;
+
+template <bool kBf16, int D, int NT, bool kBias, bool kScores>
+__global__ void __launch_bounds__(kSegThreads) paged_attention_segment_kernel(const __grid_constant__ AttnParams p) {
+  using W = Warp<kBf16, D, NT, kBias, kScores>;
+  constexpr int kFrags = NT * (D / 16);
+  static_assert(kFrags * 32 * sizeof(float4) <= W::kRing, "a warp's part fits its ring");
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ float4 stats[kSegWarps][NT][4];
+  __shared__ float2 final_stats[NT * 8];  // reference point, 1 / l
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_launch_dependents();
+  pdl_wait();
+  Cursor c;
+  c.b = blockIdx.x / p.hkv;
+  c.hx = blockIdx.x % p.hkv;
+  c.s = span_of(p, c.b);
+  c.u = c.s.u0 + warp;
+  const int n = (c.s.u1 - c.u + kSegWarps - 1) / kSegWarps;
+  Cursor ld = c;
+  W my(p, smem_u32(smem) + warp * W::kRing);
+  auto request = [&](int stage, bool any) {
+    my.request(ld, stage, any);
+    ld.u += kSegWarps;
+  };
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s) request(s, s < n);
+  my.start(c);
+  for (int i = 0, stage = 0; i < n; ++i) {
+    cp_async_wait<kStages - 2>();
+    __syncwarp();
+    const int next = stage + kStages - 1;
+    request(next >= kStages ? next - kStages : next, i + kStages - 1 < n);
+    my.add(c, stage);
+    c.u += kSegWarps;
+    if (++stage == kStages) stage = 0;
+  }
+  my.close();
+  // The ring is empty: every requested unit has been added.
+  float4* part = reinterpret_cast<float4*>(smem + warp * W::kRing);
+  __syncwarp();
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt) part[(nt * (D / 16) + dt) * 32 + lane] = my.fragment(nt, dt);
+    if (lane < 4) stats[warp][nt][lane] = my.stats(nt);
+  }
+  __syncthreads();
+  uint16_t* head0 = p.out + (static_cast<int64_t>(c.b) * p.hq + my.h0) * D;
+  for (int frag = warp; frag < kFrags; frag += kSegWarps) {
+    const int nt = frag / (D / 16), dt = frag % (D / 16);
+    float m0 = -INFINITY, m1 = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < kSegWarps; ++k) {
+      m0 = fmaxf(m0, stats[k][nt][lane & 3].x);
+      m1 = fmaxf(m1, stats[k][nt][lane & 3].z);
+    }
+    const float r0 = safe_max(m0), r1 = safe_max(m1);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+    for (int k = 0; k < kSegWarps; ++k) {
+      const float4 st = stats[k][nt][lane & 3];
+      const float4 x = reinterpret_cast<const float4*>(smem + k * W::kRing)[frag * 32 + lane];
+      const float a0 = ex2_approx(st.x - r0), a1 = ex2_approx(st.z - r1);
+      l0 = fmaf(st.y, a0, l0);
+      l1 = fmaf(st.w, a1, l1);
+      o.x = fmaf(x.x, a0, o.x);
+      o.y = fmaf(x.y, a1, o.y);
+      o.z = fmaf(x.z, a0, o.z);
+      o.w = fmaf(x.w, a1, o.w);
+    }
+    const float i0 = inv_sum(l0), i1 = inv_sum(l1);
+    const float t[4] = {o.x * i0, o.y * i1, o.z * i0, o.w * i1};
+    store_out_tile<kBf16>(p, t, head0, D, nt, dt, my.nrows);
+    if (kScores && dt == 0 && lane < 4) {
+      final_stats[nt * 8 + lane * 2] = make_float2(r0, i0);
+      final_stats[nt * 8 + lane * 2 + 1] = make_float2(r1, i1);
+    }
+  }
+  if constexpr (kScores) {
+    // All heads of the group are here.
+    __syncthreads();
+    const float* in = p.win + c.b * p.win_sb + c.hx * p.win_sh;
+    float* out = p.wout + c.b * p.wout_sb + c.hx * p.wout_sh;
+    const float* scores = p.scores + (static_cast<int64_t>(c.b) * p.hq + my.h0) * p.score_stride;
+    for (int t = threadIdx.x; t < c.s.len; t += kSegThreads) {
+      float w = in[t];
+      if (t >= c.s.lo) {
+#pragma unroll 4
+        for (int h = 0; h < my.nrows; ++h) {
+          w = fmaf(ex2_approx(scores[h * p.score_stride + t] - final_stats[h].x), final_stats[h].y, w);
+        }
+      }
+      out[t] = w;
+    }
+  }
+}
+
 // A split (sequence, kv head, tile): the runs [w0, w1] hold its pieces. Only
 // the first run can have begun before it, so the first piece is that run's
 // last one unless the run starts with it; the other pieces come first.
 struct Pieces {
-  int64_t w0, first_slot;
+  int w0, first_slot;
   int count;  // 0: one run had it all
   __device__ __forceinline__ int64_t slot(int i) const { return i == 0 ? first_slot : (w0 + i) * 2; }
 };
-__device__ __forceinline__ Pieces pieces_of(const AttnParams& p, int64_t before, int64_t all, int hx, int per) {
+__device__ __forceinline__ Pieces pieces_of(const AttnParams& p, int before, int all, int hx, int per) {
   const int heads = p.hkv * p.tiles;
-  const int64_t total = all * heads;
-  const Runs runs(p, total);
-  const int64_t s0 = before * heads + static_cast<int64_t>(hx) * (per + kStart);  // the segment's start
-  const int64_t u0 = s0 + kStart;                                                  // its first unit
-  const int64_t w0 = runs.holding(u0), w1 = runs.holding(u0 + per - 1);
-  return Pieces{w0, w0 * 2 + (runs.begin(w0) >= s0 ? 0 : 1), w0 == w1 ? 0 : static_cast<int>(w1 - w0 + 1)};
+  const Runs runs(p, all * heads);
+  const int s0 = before * heads + hx * (per + kStart);  // the segment's start
+  const int w0 = runs.holding(s0 + kStart), w1 = runs.holding(s0 + kStart + per - 1);
+  return Pieces{w0, w0 * 2 + (runs.begin(w0) >= s0 ? 0 : 1), w0 == w1 ? 0 : w1 - w0 + 1};
 }
 
 // The second kernel, CTAs (b, kv head) x y. y < join_ctas: join the pieces of
@@ -584,7 +709,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attention_join_kernel(cons
   const int b = blockIdx.x / p.hkv, kv = blockIdx.x % p.hkv;
   const Span s = span_of(p, b);
   const int per = s.u1 - s.u0;
-  int64_t before, all;
+  int before, all;
   line_sums(p, b, &before, &all);
   pdl_wait();
   pdl_launch_dependents();
@@ -732,9 +857,16 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attention_join_kernel(cons
   }
 }
 
+// A CTA per (sequence, kv head) where these fit the SMs and the tables hold at
+// most this many tokens: 16 heads x 129 tokens (D = 64) take 4.4 us that way
+// and 8.6 us through runs and join; with long tables the one CTA's units would
+// follow each other for longer than the join takes.
+constexpr int kSegTokens = 1024;
+
 struct Plan {
   int group, tiles, rows, nt, ctas, warps;
   int64_t capacity;
+  bool by_segment;
   size_t partials, stats, scores, head_stats, score_stride, bytes;
 };
 
@@ -752,11 +884,13 @@ int make_plan(int B, int hq, int hkv, int D, int width, int page_size, bool weig
   pl.nt = pl.rows > 8 ? 2 : 1;
   pl.capacity = static_cast<int64_t>(width) * page_size;
   if (pl.capacity > INT32_MAX - kUnit) pl.capacity = INT32_MAX - kUnit;
-  if (static_cast<int64_t>(B) * hkv * pl.tiles > INT32_MAX) {
-    return fail(NESO_ERR_UNSUPPORTED, "batch x heads exceeds 2^31 - 1");
-  }
   // 192 KB of rings per SM: two CTAs of four warps at D = 128, four at 64.
   const int64_t units = (pl.capacity + kUnit - 1) / kUnit * B * hkv * pl.tiles;
+  const int64_t segments = static_cast<int64_t>(B) * hkv * pl.tiles;
+  if (segments > INT32_MAX || units + segments * kStart > INT32_MAX) {
+    return fail(NESO_ERR_UNSUPPORTED, "batch x heads x table width exceeds 2^31 units of %d tokens", kUnit);
+  }
+  pl.by_segment = segments <= sm_count() && pl.capacity <= kSegTokens && pl.tiles == 1;
   const int64_t full = static_cast<int64_t>(sm_count()) * (D == 128 ? 2 : 4);
   pl.ctas = static_cast<int>(units < full ? (units > 1 ? units : 1) : full);
   pl.warps = pl.ctas * kWarps;
@@ -778,7 +912,16 @@ int make_plan(int B, int hq, int hkv, int D, int width, int page_size, bool weig
 
 template <bool kBf16, int D, int NT, bool kBias, bool kScores>
 int launch_attention(const AttnParams& p, const Plan& pl, cudaStream_t stream) {
-  constexpr int smem = kWarps * kStages * 2 * kUnit * D * 2;
+  using W = Warp<kBf16, D, NT, kBias, kScores>;
+  if (pl.by_segment) {
+    constexpr int smem = kSegWarps * W::kRing;
+    auto* kern = paged_attention_segment_kernel<kBf16, D, NT, kBias, kScores>;
+    const int rc = kernel_setup(reinterpret_cast<const void*>(kern), smem, nullptr);
+    if (rc != NESO_OK) return rc;
+    const cudaError_t e = launch_pdl(kern, dim3(p.B * p.hkv), dim3(kSegThreads), smem, stream, p);
+    return e == cudaSuccess ? ok() : cuda_fail(e, "paged_attention launch");
+  }
+  constexpr int smem = kWarps * W::kRing;
   auto* kern = paged_attention_kernel<kBf16, D, NT, kBias, kScores>;
   int rc = kernel_setup(reinterpret_cast<const void*>(kern), smem, nullptr);
   if (rc != NESO_OK) return rc;

@@ -44,6 +44,14 @@ constexpr int kStart = 4;      // cost of starting a segment, in units
 constexpr int kMinRun = 4;     // least points of a run
 constexpr float kLog2e = 1.4426950408889634f;
 
+// A segment that several runs share: its index (sequence, kv head, tile), its
+// first run, the number of runs, and the slot of the first run's piece; the
+// other runs' pieces lie in their first slots.
+struct Split {
+  int seg, w0, count, first_slot;
+  __device__ __forceinline__ int64_t slot(int i) const { return i == 0 ? first_slot : (w0 + i) * 2; }
+};
+
 struct AttnParams {
   const uint16_t* q;
   PagedCache k, v;
@@ -53,6 +61,7 @@ struct AttnParams {
   uint16_t* out;            // [B, Hq, D]
   float4* partials;         // [2 warps][NT][D/16][32]
   float4* stats;            // [2 warps][NT][4]: m, l of heads 2c, 2c+1 (log2 units)
+  Split* splits;            // [warps][2]
   float* scores;            // [B, Hq, score_stride], log2 units, when weights are wanted
   float2* head_stats;       // [B, Hq]: m, l of heads that were not split, when weights are wanted
   const float* win;
@@ -61,7 +70,7 @@ struct AttnParams {
   int B, hq, hkv, group, tiles, rows;  // tiles of `rows` query heads per kv head
   int num_pages, capacity, window, warps;
   bool whole_units;  // the page size is a multiple of kUnit
-  int join_ctas;  // CTAs per (b, kv head) that join
+  int join_ctas;
   PageDivisor page;
   float score_scale;          // scale * log2(e), or scale / softcap when scores are capped
   float softcap;
@@ -105,6 +114,7 @@ __device__ __forceinline__ void line_sums(const AttnParams& p, int b, int* befor
 // them have len + 1 points, the others len.
 struct Runs {
   int count, len, longer;
+  Runs() = default;
   __device__ __forceinline__ Runs(const AttnParams& p, int total) {
     const int most = total / kMinRun;
     count = most < 1 ? 1 : (most < p.warps ? most : p.warps);
@@ -117,6 +127,14 @@ struct Runs {
     return x < bound ? x / (len + 1) : longer + (x - bound) / len;
   }
 };
+
+// Which runs share the segment of `per` units that starts at point s0: only
+// the first of them can hold units of an earlier segment, and then its piece
+// is its last one.
+__device__ __forceinline__ Split split_of(const Runs& runs, int seg, int s0, int per) {
+  const int w0 = runs.holding(s0 + kStart), w1 = runs.holding(s0 + kStart + per - 1);
+  return Split{seg, w0, w1 - w0 + 1, w0 * 2 + (runs.begin(w0) >= s0 ? 0 : 1)};
+}
 
 // A position in the batch's order of units: sequence, (kv head, tile), unit.
 struct Cursor {
@@ -137,8 +155,9 @@ struct Cursor {
   }
 };
 
-// Run w: its first unit and how many units it has; a whole warp calls it.
-__device__ __forceinline__ int find_run(const AttnParams& p, int w, Cursor* first) {
+// Run w: its first unit, where that unit's segment starts on the line, and how
+// many units the run has; a whole warp calls it.
+__device__ __forceinline__ int find_run(const AttnParams& p, int w, Cursor* first, int* line, Runs* cut) {
   const int lane = threadIdx.x & 31;
   const int heads = p.hkv * p.tiles;
   const int cost0 = lane < p.B ? cost_of(span_of(p, lane)) : 0;
@@ -146,6 +165,7 @@ __device__ __forceinline__ int find_run(const AttnParams& p, int w, Cursor* firs
   for (int i = lane + 32; i < p.B; i += 32) sum += cost_of(span_of(p, i));
   const int total = __reduce_add_sync(0xffffffffu, sum) * heads;
   const Runs runs(p, total);
+  *cut = runs;
   if (total == 0 || w >= runs.count) return 0;
   const int from = runs.begin(w), to = runs.begin(w + 1);
   int units_from = 0, units_to = 0;
@@ -175,6 +195,7 @@ __device__ __forceinline__ int find_run(const AttnParams& p, int w, Cursor* firs
         c->s = span_of(p, c->b);
         c->hx = hx;
         c->u = c->s.u0 + unit;
+        *line = at - in;
       }
       return at - in + unit - seg * kStart;
     };
@@ -508,9 +529,21 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? 2 : 4)
 
   // Neighbouring runs go to different CTAs, so a small batch spreads over the SMs.
   const int w = warp * gridDim.x + blockIdx.x;
+  for (int b = w; b < p.B; b += p.warps) {
+    if (cost_of(span_of(p, b)) == 0) {  // no token is visible
+      uint32_t* dst = reinterpret_cast<uint32_t*>(p.out + static_cast<int64_t>(b) * p.hq * D);
+      for (int i = lane; i < p.hq * (D / 2); i += 32) dst[i] = 0u;
+    }
+  }
   Cursor ld;
-  const int n = find_run(p, w, &ld);
-  if (n == 0) return;
+  Runs runs;
+  int line = 0;
+  const int n = find_run(p, w, &ld, &line, &runs);
+  Split first_split{0, 0, 0, 0}, started{0, 0, 0, 0};
+  if (n == 0) {
+    if (lane == 0) p.splits[w * 2] = p.splits[w * 2 + 1] = started;
+    return;
+  }
   Cursor c = ld;
   W my(p, smem_u32(smem) + warp * W::kRing);
   auto request = [&](int stage, bool any) {
@@ -558,6 +591,11 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? 2 : 4)
             }
           }
         } else {
+          if (nt == 0) {
+            const Split sp = split_of(runs, c.b * p.hkv * p.tiles + c.hx, line, c.s.u1 - c.s.u0);
+            if (first_piece) first_split = sp;
+            if (sp.w0 == w) started = sp;
+          }
 #pragma unroll
           for (int dt = 0; dt < D / 16; ++dt) p.partials[((slot * NT + nt) * (D / 16) + dt) * 32 + lane] = my.fragment(nt, dt);
           if (lane < 4) p.stats[(slot * NT + nt) * 4 + lane] = my.stats(nt);
@@ -565,9 +603,14 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? 2 : 4)
       }
       fresh = true;
       first_piece = false;
+      line += c.s.u1 - c.s.u0 + kStart;
     }
     c.next(p);
     if (++stage == kStages) stage = 0;
+  }
+  if (lane == 0) {
+    p.splits[w * 2] = first_split;
+    p.splits[w * 2 + 1] = started;
   }
 }
 
@@ -673,119 +716,217 @@ __global__ void __launch_bounds__(kSegThreads) paged_attention_segment_kernel(co
   }
 }
 
-// A split (sequence, kv head, tile): the runs [w0, w1] hold its pieces. Only
-// the first run can have begun before it, so the first piece is that run's
-// last one unless the run starts with it; the other pieces come first.
-struct Pieces {
-  int w0, first_slot;
-  int count;  // 0: one run had it all
-  __device__ __forceinline__ int64_t slot(int i) const { return i == 0 ? first_slot : (w0 + i) * 2; }
-};
-__device__ __forceinline__ Pieces pieces_of(const AttnParams& p, int before, int all, int hx, int per) {
-  const int heads = p.hkv * p.tiles;
-  const Runs runs(p, all * heads);
-  const int s0 = before * heads + hx * (per + kStart);  // the segment's start
-  const int w0 = runs.holding(s0 + kStart), w1 = runs.holding(s0 + kStart + per - 1);
-  return Pieces{w0, w0 * 2 + (runs.begin(w0) >= s0 ? 0 : 1), w0 == w1 ? 0 : w1 - w0 + 1};
-}
-
-// The second kernel, CTAs (b, kv head) x y. y < join_ctas: join the pieces of
-// split segments (and write zeros where no token is visible); each warp takes
-// one fragment of 16 d x 8 heads and every kParts-th piece, and the warps of a
-// fragment add up in shared memory in a fixed order. Other y, when the weights
-// are wanted: kWeightTokens tokens of
+// The second kernel. CTAs below p.join_ctas join the pieces of split segments.
+// Each takes consecutive runs, as many as make some 300 CTAs, and the segments
+// that start in them. A warp joins kPairFrags fragments (of 16 d x 8 heads) at
+// a time of a segment in two or three pieces, one fragment of a segment in more;
+// what matters is that all it reads is requested at once. The runs of a segment
+// of more than kFewPieces pieces fill several CTAs: those take its fragments in
+// turn, each warp an equal part of the pieces. Everything adds up in a fixed
+// order. The other CTAs, when the weights are wanted, take kWeightTokens tokens
+// of one (sequence, kv head):
 //   weights_out[t] = weights_in[t] + sum_h exp2(s[h, t] - m[h]) / l[h].
-constexpr int kJoinWarps = 16;
+constexpr int kJoinWarps = 8;
 constexpr int kJoinThreads = kJoinWarps * 32;
+constexpr int kPairFrags = 2;
+constexpr int kFewPieces = 16;
+constexpr int kJoinBatch = 4;  // pieces that a warp has requested
 constexpr int kWeightTokens = 1024;
 constexpr int kWeightSteps = kWeightTokens / kJoinThreads;
+constexpr int kWeightHeads = 4;  // heads whose scores a thread has requested
 
-template <bool kBf16, int D, int NT, bool kScores>
-__global__ void __launch_bounds__(kJoinThreads) paged_attention_join_kernel(const __grid_constant__ AttnParams p) {
-  constexpr int kFrags = NT * (D / 16);
-  __shared__ float4 acc[kJoinWarps][32];
-  __shared__ float4 sums[kJoinWarps][4];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int b = blockIdx.x / p.hkv, kv = blockIdx.x % p.hkv;
-  const Span s = span_of(p, b);
-  const int per = s.u1 - s.u0;
-  int before, all;
-  line_sums(p, b, &before, &all);
-  pdl_wait();
-  pdl_launch_dependents();
+struct JoinShared {
+  float4 acc[kJoinWarps][32];
+  float4 sums[kJoinWarps][4];
+};
 
-  if (!kScores || blockIdx.y < p.join_ctas) {
-    const int frags = kFrags / p.join_ctas;  // per CTA
-    const int parts = kJoinWarps / frags;
-    const int part = warp / frags, frag = blockIdx.y * frags + warp % frags;
-    const int nt = frag / (D / 16), dt = frag % (D / 16);
-    for (int tile = 0; tile < p.tiles; ++tile) {
-      const int h0 = kv * p.group + tile * p.rows;
-      const int nrows = p.group - tile * p.rows < p.rows ? p.group - tile * p.rows : p.rows;
-      uint16_t* head0 = p.out + (static_cast<int64_t>(b) * p.hq + h0) * D;
-      if (per == 0) {
-        uint32_t* dst = reinterpret_cast<uint32_t*>(head0);
-        for (int i = blockIdx.y * kJoinThreads + threadIdx.x; i < nrows * D / 2; i += p.join_ctas * kJoinThreads) dst[i] = 0u;
-        continue;
-      }
-      const Pieces pc = pieces_of(p, before, all, kv * p.tiles + tile, per);
-      if (pc.count == 0) continue;
-      float m0 = -INFINITY, m1 = -INFINITY;
-      for (int i = lane >> 2; i < pc.count; i += 8) {
-        const float4 st = p.stats[(pc.slot(i) * NT + nt) * 4 + (lane & 3)];
-        m0 = fmaxf(m0, st.x);
-        m1 = fmaxf(m1, st.z);
-      }
+// Statistics and fragment of some pieces, added up one after the other.
+struct Joined {
+  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  __device__ __forceinline__ void add(const float4& st, const float4& x) {
+    const float n0 = fmaxf(m0, st.x), n1 = fmaxf(m1, st.z);
+    const float a0 = ex2_approx(m0 - safe_max(n0)), a1 = ex2_approx(m1 - safe_max(n1));
+    const float b0 = ex2_approx(st.x - safe_max(n0)), b1 = ex2_approx(st.z - safe_max(n1));
+    l0 = fmaf(st.y, b0, l0 * a0);
+    l1 = fmaf(st.w, b1, l1 * a1);
+    o.x = fmaf(x.x, b0, o.x * a0);
+    o.y = fmaf(x.y, b1, o.y * a1);
+    o.z = fmaf(x.z, b0, o.z * a0);
+    o.w = fmaf(x.w, b1, o.w * a1);
+    m0 = n0;
+    m1 = n1;
+  }
+};
+
+template <int D, int NT>
+__device__ __forceinline__ void add_pieces(const AttnParams& p, const Split& sp, int frag, int first, int step, Joined& j) {
+  const int lane = threadIdx.x & 31;
+  const int nt = frag / (D / 16), dt = frag % (D / 16);
+  for (int i0 = first; i0 < sp.count; i0 += kJoinBatch * step) {
+    float4 st[kJoinBatch], x[kJoinBatch];
 #pragma unroll
-      for (int d = 4; d < 32; d <<= 1) {
-        m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, d));
-        m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, d));
+    for (int k = 0; k < kJoinBatch; ++k) {
+      const int i = i0 + k * step;
+      if (i < sp.count) {
+        const int64_t slot = sp.slot(i) * NT + nt;
+        st[k] = p.stats[slot * 4 + (lane & 3)];
+        x[k] = p.partials[(slot * (D / 16) + dt) * 32 + lane];
       }
-      const float r0 = safe_max(m0), r1 = safe_max(m1);
-      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-      float l0 = 0.f, l1 = 0.f;
-#pragma unroll 4
-      for (int i = part; i < pc.count; i += parts) {
-        const int64_t slot = pc.slot(i) * NT + nt;
-        const float4 st = p.stats[slot * 4 + (lane & 3)];
-        const float4 x = p.partials[(slot * (D / 16) + dt) * 32 + lane];
-        const float a0 = ex2_approx(st.x - r0), a1 = ex2_approx(st.z - r1);
-        l0 = fmaf(st.y, a0, l0);
-        l1 = fmaf(st.w, a1, l1);
-        o.x = fmaf(x.x, a0, o.x);
-        o.y = fmaf(x.y, a1, o.y);
-        o.z = fmaf(x.z, a0, o.z);
-        o.w = fmaf(x.w, a1, o.w);
-      }
-      if (parts > 1) {
-        __syncthreads();  // the last tile's sums have been read
-        acc[warp][lane] = o;
-        if (lane < 4) sums[warp][lane] = make_float4(l0, l1, 0.f, 0.f);
-        __syncthreads();
-        if (part > 0) continue;
-        for (int k = 1; k < parts; ++k) {
-          const float4 x = acc[k * frags + warp][lane], y = sums[k * frags + warp][lane & 3];
-          o.x += x.x;
-          o.y += x.y;
-          o.z += x.z;
-          o.w += x.w;
-          l0 += y.x;
-          l1 += y.y;
+    }
+#pragma unroll
+    for (int k = 0; k < kJoinBatch; ++k) {
+      if (i0 + k * step < sp.count) j.add(st[k], x[k]);
+    }
+  }
+}
+
+template <int D>
+constexpr int join_runs() {
+  return D == 64 ? 8 : 4;
+}
+
+template <bool kBf16, int D, int NT>
+__device__ __forceinline__ void join_segments(const AttnParams& p, JoinShared& sh) {
+  constexpr int kJoinRuns = join_runs<D>();
+  constexpr int kFrags = NT * (D / 16);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int heads = p.hkv * p.tiles;
+  auto write = [&](const Split& sp, int frag, const Joined& j) {
+    const int b = sp.seg / heads, hx = sp.seg - b * heads;
+    const int kv = hx / p.tiles, tile = hx - kv * p.tiles;
+    const int nrows = p.group - tile * p.rows < p.rows ? p.group - tile * p.rows : p.rows;
+    const float i0 = inv_sum(j.l0), i1 = inv_sum(j.l1);
+    const float t[4] = {j.o.x * i0, j.o.y * i1, j.o.z * i0, j.o.w * i1};
+    store_out_tile<kBf16>(p, t, p.out + (static_cast<int64_t>(b) * p.hq + kv * p.group + tile * p.rows) * D, D,
+                          frag / (D / 16), frag % (D / 16), nrows);
+  };
+  // Lane i has run i / 2's first piece (even) or the segment that starts in it (odd).
+  const int run0 = blockIdx.x * kJoinRuns;
+  Split mine{0, 0, 0, 0};
+  if (lane < 2 * kJoinRuns && run0 + lane / 2 < p.warps) mine = p.splits[run0 * 2 + lane];
+  auto split = [&](int i) {
+    return Split{__shfl_sync(0xffffffffu, mine.seg, i), __shfl_sync(0xffffffffu, mine.w0, i),
+                 __shfl_sync(0xffffffffu, mine.count, i), __shfl_sync(0xffffffffu, mine.first_slot, i)};
+  };
+  const uint32_t few = __ballot_sync(0xffffffffu, (lane & 1) && mine.count > 1 && mine.count <= kFewPieces);
+  int task = 0;
+  for (uint32_t left = few; left != 0; left &= left - 1) {
+    const Split sp = split(__ffs(left) - 1);
+    if (sp.count <= 3) {
+      for (int frag0 = 0; frag0 < kFrags; frag0 += kPairFrags, ++task) {
+        if (task % kJoinWarps != warp) continue;
+        const int nt = frag0 / (D / 16);  // kPairFrags divides D / 16
+        float4 st[3], x[3][kPairFrags];
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+          if (i < sp.count) {
+            const int64_t slot = sp.slot(i) * NT;
+            st[i] = p.stats[(slot + nt) * 4 + (lane & 3)];
+#pragma unroll
+            for (int f = 0; f < kPairFrags; ++f) x[i][f] = p.partials[(slot * (D / 16) + frag0 + f) * 32 + lane];
+          }
+        }
+#pragma unroll
+        for (int f = 0; f < kPairFrags; ++f) {
+          Joined j;
+#pragma unroll
+          for (int i = 0; i < 3; ++i) {
+            if (i < sp.count) j.add(st[i], x[i][f]);
+          }
+          write(sp, frag0 + f, j);
         }
       }
-      const float i0 = inv_sum(l0), i1 = inv_sum(l1);
-      const float t[4] = {o.x * i0, o.y * i1, o.z * i0, o.w * i1};
-      store_out_tile<kBf16>(p, t, head0, D, nt, dt, nrows);
+      continue;
     }
+    for (int frag = 0; frag < kFrags; ++frag, ++task) {
+      if (task % kJoinWarps != warp) continue;
+      Joined j;
+      add_pieces<D, NT>(p, sp, frag, 0, 1, j);
+      write(sp, frag, j);
+    }
+  }
+  uint32_t many = __ballot_sync(0xffffffffu, !(lane & 1) && mine.count > kFewPieces && run0 + lane / 2 != mine.w0);
+  int before = -1;
+  for (; many != 0; many &= many - 1) {
+    const Split sp = split(__ffs(many) - 1);
+    if (sp.seg == before) continue;
+    before = sp.seg;
+    const int cta0 = (sp.w0 + 1) / kJoinRuns, ctas = (sp.w0 + sp.count - 1) / kJoinRuns - cta0 + 1;
+    for (int frag = blockIdx.x - cta0; frag < kFrags; frag += ctas) {
+      Joined j;
+      add_pieces<D, NT>(p, sp, frag, warp, kJoinWarps, j);
+      __syncthreads();  // the last fragment's sums have been read
+      sh.acc[warp][lane] = j.o;
+      if (lane < 4) sh.sums[warp][lane] = make_float4(j.m0, j.l0, j.m1, j.l1);
+      __syncthreads();
+      if (warp == 0) {
+#pragma unroll
+        for (int k = 1; k < kJoinWarps; ++k) j.add(sh.sums[k][lane & 3], sh.acc[k][lane]);
+        write(sp, frag, j);
+      }
+    }
+  }
+}
+
+// Reference point and 1 / l of the NT * 8 heads of one tile, into shared memory.
+template <int NT>
+__device__ __forceinline__ void tile_stats(const AttnParams& p, const Split& sp, int64_t head, int nrows, float2* stat) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warp >= NT) return;
+  // Lane quads take two heads each of every eighth piece.
+  const int col = warp * 8 + (lane & 3) * 2;
+  Joined j;
+  const float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (sp.count == 1) {
+    float2 st[2] = {make_float2(-INFINITY, 0.f), make_float2(-INFINITY, 0.f)};
+    for (int k = 0; k < 2; ++k) {
+      if (col + k < nrows) st[k] = p.head_stats[head + col + k];
+    }
+    j.m0 = st[0].x;
+    j.l0 = st[0].y;
+    j.m1 = st[1].x;
+    j.l1 = st[1].y;
+  } else {
+#pragma unroll 4
+    for (int i = lane >> 2; i < sp.count; i += 8) j.add(p.stats[(sp.slot(i) * NT + warp) * 4 + (lane & 3)], none);
+#pragma unroll
+    for (int d = 4; d < 32; d <<= 1) {
+      const float4 other = make_float4(__shfl_xor_sync(0xffffffffu, j.m0, d), __shfl_xor_sync(0xffffffffu, j.l0, d),
+                                       __shfl_xor_sync(0xffffffffu, j.m1, d), __shfl_xor_sync(0xffffffffu, j.l1, d));
+      j.add(other, none);
+    }
+  }
+  if (lane < 4) {
+    stat[col] = make_float2(safe_max(j.m0), inv_sum(j.l0));
+    stat[col + 1] = make_float2(safe_max(j.m1), inv_sum(j.l1));
+  }
+}
+
+template <bool kBf16, int D, int NT, bool kScores>
+__global__ void __launch_bounds__(kJoinThreads, 2) paged_attention_join_kernel(const __grid_constant__ AttnParams p) {
+  __shared__ JoinShared sh;
+  if (!kScores || blockIdx.x < p.join_ctas) {
+    pdl_wait();
+    pdl_launch_dependents();
+    join_segments<kBf16, D, NT>(p, sh);
     return;
   }
-
   if constexpr (kScores) {
-    float2* stat = reinterpret_cast<float2*>(&sums[0][0]);  // 16 heads: reference point, 1 / l
+    const int pair = (blockIdx.x - p.join_ctas) % (p.B * p.hkv), chunk = (blockIdx.x - p.join_ctas) / (p.B * p.hkv);
+    const int b = pair / p.hkv, kv = pair % p.hkv;
+    const Span s = span_of(p, b);
+    const int per = s.u1 - s.u0, heads = p.hkv * p.tiles;
+    int before, all;
+    line_sums(p, b, &before, &all);
+    const Runs runs(p, all * heads);
+    pdl_wait();
+    pdl_launch_dependents();
+    if (chunk * kWeightTokens >= s.len) return;
+    float2* stat = reinterpret_cast<float2*>(&sh.sums[0][0]);
     const float* in = p.win + b * p.win_sb + kv * p.win_sh;
     float* out = p.wout + b * p.wout_sb + kv * p.wout_sh;
-    const int begin = (blockIdx.y - p.join_ctas) * kWeightTokens + threadIdx.x;
-    if (begin - static_cast<int>(threadIdx.x) >= s.len) return;
+    const int begin = chunk * kWeightTokens + threadIdx.x;
     float w[kWeightSteps];
 #pragma unroll
     for (int i = 0; i < kWeightSteps; ++i) {
@@ -796,56 +937,29 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attention_join_kernel(cons
       const int h0 = kv * p.group + tile * p.rows;
       const int nrows = p.group - tile * p.rows < p.rows ? p.group - tile * p.rows : p.rows;
       const int64_t head = static_cast<int64_t>(b) * p.hq + h0;
-      const Pieces pc = pieces_of(p, before, all, kv * p.tiles + tile, per);
-      __syncthreads();
-      if (warp < NT) {
-        // Lane quads add up the pieces of two heads each.
-        const int col = warp * 8 + (lane & 3) * 2;
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-        if (pc.count == 0) {
-          for (int j = 0; j < 2; ++j) {
-            if (col + j < nrows) {
-              const float2 st = p.head_stats[head + col + j];
-              m[j] = st.x;
-              l[j] = st.y;
-            }
-          }
-        } else {
-          for (int i = lane >> 2; i < pc.count; i += 8) {
-            const float4 st = p.stats[(pc.slot(i) * NT + warp) * 4 + (lane & 3)];
-            m[0] = fmaxf(m[0], st.x);
-            m[1] = fmaxf(m[1], st.z);
-          }
+      const float* scores = p.scores + head * p.score_stride;
+      const Split sp = split_of(runs, 0, before * heads + (kv * p.tiles + tile) * (per + kStart), per);
+      for (int g = 0; g < nrows; g += kWeightHeads) {
+        float x[kWeightHeads][kWeightSteps];
 #pragma unroll
-          for (int d = 4; d < 32; d <<= 1) {
-            m[0] = fmaxf(m[0], __shfl_xor_sync(0xffffffffu, m[0], d));
-            m[1] = fmaxf(m[1], __shfl_xor_sync(0xffffffffu, m[1], d));
-          }
-          for (int i = lane >> 2; i < pc.count; i += 8) {
-            const float4 st = p.stats[(pc.slot(i) * NT + warp) * 4 + (lane & 3)];
-            l[0] = fmaf(st.y, ex2_approx(st.x - safe_max(m[0])), l[0]);
-            l[1] = fmaf(st.w, ex2_approx(st.z - safe_max(m[1])), l[1]);
-          }
+        for (int h = 0; h < kWeightHeads; ++h) {
 #pragma unroll
-          for (int d = 4; d < 32; d <<= 1) {
-            l[0] += __shfl_xor_sync(0xffffffffu, l[0], d);
-            l[1] += __shfl_xor_sync(0xffffffffu, l[1], d);
+          for (int i = 0; i < kWeightSteps; ++i) {
+            const int t = begin + i * kJoinThreads;
+            x[h][i] = g + h < nrows && t >= s.lo && t < s.len ? scores[(g + h) * p.score_stride + t] : -INFINITY;
           }
         }
-        if (lane < 4) {
-          stat[col] = make_float2(safe_max(m[0]), inv_sum(l[0]));
-          stat[col + 1] = make_float2(safe_max(m[1]), inv_sum(l[1]));
+        if (g == 0) {  // while the scores are on their way
+          __syncthreads();
+          tile_stats<NT>(p, sp, head, nrows, stat);
+          __syncthreads();
         }
-      }
-      __syncthreads();
-#pragma unroll 4
-      for (int h = 0; h < nrows; ++h) {
-        const float* row = p.scores + (head + h) * p.score_stride;
-        const float2 st = stat[h];
 #pragma unroll
-        for (int i = 0; i < kWeightSteps; ++i) {
-          const int t = begin + i * kJoinThreads;
-          if (t >= s.lo && t < s.len) w[i] = fmaf(ex2_approx(row[t] - st.x), st.y, w[i]);
+        for (int h = 0; h < kWeightHeads; ++h) {
+          if (g + h >= nrows) break;
+          const float2 st = stat[g + h];
+#pragma unroll
+          for (int i = 0; i < kWeightSteps; ++i) w[i] = fmaf(ex2_approx(x[h][i] - st.x), st.y, w[i]);
         }
       }
     }
@@ -867,7 +981,7 @@ struct Plan {
   int group, tiles, rows, nt, ctas, warps;
   int64_t capacity;
   bool by_segment;
-  size_t partials, stats, scores, head_stats, score_stride, bytes;
+  size_t partials, stats, splits, scores, head_stats, score_stride, bytes;
 };
 
 size_t round_up(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
@@ -898,6 +1012,8 @@ int make_plan(int B, int hq, int hkv, int D, int width, int page_size, bool weig
   size_t at = round_up(static_cast<size_t>(pl.warps) * 2 * pl.nt * (D / 16) * 32 * sizeof(float4));
   pl.stats = at;
   at += round_up(static_cast<size_t>(pl.warps) * 2 * pl.nt * 4 * sizeof(float4));
+  pl.splits = at;
+  at += round_up(static_cast<size_t>(pl.warps) * 2 * sizeof(Split));
   if (weights) {
     pl.score_stride = static_cast<size_t>((pl.capacity + kUnit - 1) / kUnit * kUnit);
     pl.scores = at;
@@ -927,9 +1043,10 @@ int launch_attention(const AttnParams& p, const Plan& pl, cudaStream_t stream) {
   if (rc != NESO_OK) return rc;
   cudaError_t e = launch_pdl(kern, dim3(pl.ctas), dim3(kThreads), smem, stream, p);
   if (e != cudaSuccess) return cuda_fail(e, "paged_attention launch");
-  const int64_t chunks = kScores ? (pl.capacity + kWeightTokens - 1) / kWeightTokens : 0;
-  e = launch_pdl(paged_attention_join_kernel<kBf16, D, NT, kScores>,
-                 dim3(p.B * p.hkv, static_cast<unsigned>(p.join_ctas + chunks)), dim3(kJoinThreads), 0, stream, p);
+  const int64_t pairs = static_cast<int64_t>(p.B) * p.hkv;
+  const int64_t weight_ctas = kScores ? (pl.capacity + kWeightTokens - 1) / kWeightTokens * pairs : 0;
+  e = launch_pdl(paged_attention_join_kernel<kBf16, D, NT, kScores>, dim3(static_cast<unsigned>(p.join_ctas + weight_ctas)),
+                 dim3(kJoinThreads), 0, stream, p);
   if (e != cudaSuccess) return cuda_fail(e, "paged_attention join launch");
   return ok();
 }
@@ -1008,8 +1125,9 @@ int neso_paged_attention(const void* q, const void* k_cache, const void* v_cache
                 static_cast<long long>(workspace == nullptr ? 0 : workspace_bytes), static_cast<long long>(pl.bytes));
   }
   if (!aligned16(workspace)) return fail(NESO_ERR_MISALIGNED, "workspace is not 16-byte aligned");
-  if (weights_out != nullptr && (pl.capacity + kWeightTokens - 1) / kWeightTokens > 65000) {
-    return fail(NESO_ERR_UNSUPPORTED, "weights are limited to tables of 65000 x %d tokens", kWeightTokens);
+  if (weights_out != nullptr &&
+      (pl.capacity + kWeightTokens - 1) / kWeightTokens * (static_cast<int64_t>(B) * Hkv) > INT32_MAX - pl.warps) {
+    return fail(NESO_ERR_UNSUPPORTED, "batch x kv heads x table width is too large for weights");
   }
   p.q = static_cast<const uint16_t*>(q);
   p.tables = block_tables;
@@ -1019,6 +1137,7 @@ int neso_paged_attention(const void* q, const void* k_cache, const void* v_cache
   char* ws = static_cast<char*>(workspace);
   p.partials = reinterpret_cast<float4*>(ws + pl.partials);
   p.stats = reinterpret_cast<float4*>(ws + pl.stats);
+  p.splits = reinterpret_cast<Split*>(ws + pl.splits);
   p.scores = reinterpret_cast<float*>(ws + pl.scores);
   p.head_stats = reinterpret_cast<float2*>(ws + pl.head_stats);
   p.win = weights_in;
@@ -1042,10 +1161,8 @@ int neso_paged_attention(const void* q, const void* k_cache, const void* v_cache
   p.window = window;
   p.warps = pl.warps;
   p.whole_units = page_size % kUnit == 0;
-  // With few (sequence, kv head) pairs each has many pieces and the SMs are
-  // idle: a CTA per fragment then.
-  const int frags = pl.nt * (D / 16);
-  p.join_ctas = static_cast<int64_t>(B) * Hkv * frags <= 2 * sm_count() ? frags : 1;
+  const int join = D == 64 ? join_runs<64>() : join_runs<128>();
+  p.join_ctas = (pl.warps + join - 1) / join;
   p.page = page_divisor(static_cast<uint32_t>(page_size));
   p.score_scale = softcap > 0.f ? scale / softcap : scale * kLog2e;
   p.softcap = softcap;

@@ -255,50 +255,58 @@ __device__ __forceinline__ void cluster_barrier_relaxed() {
 }
 
 struct EvictShared {
-  int hist[kCopiesOfHist * kHistPitch];
+  int hist[2][kCopiesOfHist * kHistPitch];
   alignas(16) int total[kDigits];
   int warp_sum[2][kEvictWarps];
   int slice[2];  // long sequences: kept for sure and ties of this CTA's slice
-  int pick[3];
 };
 // Short sequences, dynamic shared memory: the weights (padded), then the kept
 // tokens and their weights.
 constexpr int kSelectBytes = (kShortLen + kEvictThreads + kShortLen) * 4;
 
 // Count this thread's digit, in its copy of the histogram.
-__device__ __forceinline__ void count_digit(EvictShared& sh, uint32_t key, uint32_t prefix, int shift) {
+__device__ __forceinline__ void count_digit(int* hist, uint32_t key, uint32_t prefix, int shift) {
   if (shift == 32 - kDigitBits || ((key ^ prefix) >> (shift + kDigitBits)) == 0) {
-    atomicAdd(&sh.hist[(threadIdx.x % kCopiesOfHist) * kHistPitch + ((key >> shift) & (kDigits - 1))], 1);
+    atomicAdd(&hist[(threadIdx.x % kCopiesOfHist) * kHistPitch + ((key >> shift) & (kDigits - 1))], 1);
   }
 }
 
-// From total[]: the digit that holds the need-th largest key (pick[0]), how
-// many of its keys are wanted (pick[1]) and how many it has (pick[2]). Warp 0.
-__device__ __forceinline__ void pick_digit(EvictShared& sh, int need) {
+// The digit that holds the need-th largest key, how many of its keys are wanted
+// and how many it has. Every warp works it out for itself.
+struct Pick {
+  int digit, wanted, has;
+};
+__device__ __forceinline__ Pick pick_digit(const int* total, int need) {
   constexpr int kPer = kDigits / 32;
   const int lane = threadIdx.x & 31;
-  int mine = 0;  // digits from the largest down, kPer to a lane
+  int of[kPer];  // digits from the largest down, kPer to a lane
+  int mine = 0;
 #pragma unroll
-  for (int j = 0; j < kPer; ++j) mine += sh.total[kDigits - 1 - (lane * kPer + j)];
+  for (int j = 0; j < kPer; ++j) {
+    of[j] = total[kDigits - 1 - (lane * kPer + j)];
+    mine += of[j];
+  }
   int incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int x = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += x;
   }
+  const uint32_t reached = __ballot_sync(0xffffffffu, need <= incl);
   int before = incl - mine;
-  if (before < need && need <= incl) {
-    for (int j = 0; j < kPer; ++j) {
-      const int digit = kDigits - 1 - (lane * kPer + j);
-      if (before + sh.total[digit] >= need) {
-        sh.pick[0] = digit;
-        sh.pick[1] = need - before;
-        sh.pick[2] = sh.total[digit];
-        break;
-      }
-      before += sh.total[digit];
+  Pick pick{0, 0, 0};
+  bool found = false;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    if (!found && before + of[j] >= need) {
+      pick = Pick{kDigits - 1 - (lane * kPer + j), need - before, of[j]};
+      found = true;
     }
+    before += of[j];
   }
+  const int src = __ffs(reached) - 1;
+  return Pick{__shfl_sync(0xffffffffu, pick.digit, src), __shfl_sync(0xffffffffu, pick.wanted, src),
+              __shfl_sync(0xffffffffu, pick.has, src)};
 }
 
 // What a selection found: keys above `bound` are kept, and the first `ties`
@@ -329,10 +337,17 @@ __global__ void __launch_bounds__(kEvictThreads, 2) kv_select_kernel(const __gri
     }
   };
 
+  const float* win = p.win + b * p.win_sb + h * p.win_sh;
+  // A short sequence's weights are requested along with its length.
+  float early[kItems];
+#pragma unroll
+  for (int i = 0; i < kItems; ++i) {
+    const int t = i * kEvictThreads + tid;
+    early[i] = rank == 0 && t < p.capacity ? win[t] : 0.f;
+  }
   int len = p.lens[b];
   len = len < 0 ? 0 : (len > p.capacity ? p.capacity : len);
   const int keep = len < p.budget ? len : p.budget;
-  const float* win = p.win + b * p.win_sb + h * p.win_sh;
   float* wout = p.wout + b * p.wout_sb + h * p.wout_sh;
   int32_t* kept = p.kept + (static_cast<int64_t>(b) * p.hkv + h) * p.budget;
   // Candidates [lo, hi) are ranked; tokens outside are kept.
@@ -346,40 +361,49 @@ __global__ void __launch_bounds__(kEvictThreads, 2) kv_select_kernel(const __gri
     // Thread i takes tokens [i * items, (i + 1) * items), through shared
     // memory (one word of padding after 16) so that the loads are coalesced.
     const int items = (len + kEvictThreads - 1) / kEvictThreads;
-    for (int t = tid; t < len; t += kEvictThreads) list[t + (t >> 4)] = __float_as_int(win[t]);
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      const int t = i * kEvictThreads + tid;
+      if (i >= items) break;
+      if (t < len) list[t + (t >> 4)] = __float_as_int(early[i]);
+    }
+    for (int i = tid; i < 2 * kCopiesOfHist * kHistPitch; i += kEvictThreads) sh.hist[0][i] = 0;
     __syncthreads();
     int bits[kItems];
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {
       const int t = tid * items + i;
-      bits[i] = i < items && t < len ? list[t + (t >> 4)] : 0;
+      if (i >= items) break;
+      bits[i] = t < len ? list[t + (t >> 4)] : 0;
     }
     auto key_of = [&](int i) { return weight_key(__int_as_float(bits[i])); };
     Selected sel{0xffffffffu, 0};
     if (wanted > 0) {
       uint32_t prefix = 0;
       int need = wanted;
-      for (int shift = 32 - kDigitBits; shift >= 0; shift -= kDigitBits) {
-        for (int i = tid; i < kCopiesOfHist * kHistPitch; i += kEvictThreads) sh.hist[i] = 0;
-        __syncthreads();
+      for (int shift = 32 - kDigitBits, pass = 0; shift >= 0; shift -= kDigitBits, ++pass) {
+        int* hist = sh.hist[pass & 1];
+        int* next = sh.hist[~pass & 1];
 #pragma unroll
         for (int i = 0; i < kItems; ++i) {
           const int t = tid * items + i;
-          if (i < items && t >= lo && t < hi) count_digit(sh, key_of(i), prefix, shift);
+          if (i >= items) break;
+          if (t >= lo && t < hi) count_digit(hist, key_of(i), prefix, shift);
         }
         __syncthreads();
         if (tid < kDigits) {
           int sum = 0;
 #pragma unroll
-          for (int c = 0; c < kCopiesOfHist; ++c) sum += sh.hist[c * kHistPitch + tid];
+          for (int c = 0; c < kCopiesOfHist; ++c) sum += hist[c * kHistPitch + tid];
           sh.total[tid] = sum;
+        } else if (pass > 0) {
+          for (int i = tid - kDigits; i < kCopiesOfHist * kHistPitch; i += kEvictThreads - kDigits) next[i] = 0;
         }
         __syncthreads();
-        if (warp == 0) pick_digit(sh, need);
-        __syncthreads();
-        prefix |= static_cast<uint32_t>(sh.pick[0]) << shift;
-        need = sh.pick[1];
-        if (need == sh.pick[2]) {
+        const Pick pick = pick_digit(sh.total, need);
+        prefix |= static_cast<uint32_t>(pick.digit) << shift;
+        need = pick.wanted;
+        if (need == pick.has) {
           // Every key of this digit is wanted: the ones from prefix up. (prefix
           // is not 0: then all candidates would be kept.)
           prefix -= 1;
@@ -394,7 +418,8 @@ __global__ void __launch_bounds__(kEvictThreads, 2) kv_select_kernel(const __gri
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {
       const int t = tid * items + i;
-      if (i < items && t < len) {
+      if (i >= items) break;
+      if (t < len) {
         const bool in = t >= lo && t < hi;
         mine += (!in || (wanted > 0 && key_of(i) > sel.bound)) ? 1u : 0u;
         mine += (in && sel.ties > 0 && key_of(i) == sel.bound) ? 0x10000u : 0u;
@@ -415,7 +440,8 @@ __global__ void __launch_bounds__(kEvictThreads, 2) kv_select_kernel(const __gri
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {
       const int t = tid * items + i;
-      if (i < items && t < len) {
+      if (i >= items) break;
+      if (t < len) {
         const bool in = t >= lo && t < hi;
         const bool yes = !in || (wanted > 0 && key_of(i) > sel.bound);
         const bool tie = in && sel.ties > 0 && key_of(i) == sel.bound;
@@ -440,29 +466,29 @@ __global__ void __launch_bounds__(kEvictThreads, 2) kv_select_kernel(const __gri
     int need = wanted;
     if (need > 0) {
       prefix = 0;
+      int* hist = sh.hist[0];
       for (int shift = 32 - kDigitBits; shift >= 0; shift -= kDigitBits) {
-        for (int i = tid; i < kCopiesOfHist * kHistPitch; i += kEvictThreads) sh.hist[i] = 0;
+        for (int i = tid; i < kCopiesOfHist * kHistPitch; i += kEvictThreads) hist[i] = 0;
         __syncthreads();
-        for (int t = max(t0, lo) + tid; t < min(t1, hi); t += kEvictThreads) count_digit(sh, weight_key(win[t]), prefix, shift);
+        for (int t = max(t0, lo) + tid; t < min(t1, hi); t += kEvictThreads) count_digit(hist, weight_key(win[t]), prefix, shift);
         __syncthreads();
         if (tid < kDigits) {
           int sum = 0;
 #pragma unroll
-          for (int c = 0; c < kCopiesOfHist; ++c) sum += sh.hist[c * kHistPitch + tid];
-          sh.hist[tid] = sum;  // the first copy: only this thread reads and writes column tid
+          for (int c = 0; c < kCopiesOfHist; ++c) sum += hist[c * kHistPitch + tid];
+          hist[tid] = sum;  // the first copy: only this thread reads and writes column tid
         }
         sync_cluster();
         if (tid < kDigits) {
           int sum = 0;
-          for (int r = 0; r < ctas; ++r) sum += ctas > 1 ? cluster.map_shared_rank(sh.hist, r)[tid] : sh.hist[tid];
+          for (int r = 0; r < ctas; ++r) sum += ctas > 1 ? cluster.map_shared_rank(hist, r)[tid] : hist[tid];
           sh.total[tid] = sum;
         }
-        __syncthreads();
-        if (warp == 0) pick_digit(sh, need);
-        sync_cluster();  // pick is there, and every CTA has read the counts
-        prefix |= static_cast<uint32_t>(sh.pick[0]) << shift;
-        need = sh.pick[1];
-        if (need == sh.pick[2]) {
+        sync_cluster();  // the totals are there, and every CTA has read the counts
+        const Pick pick = pick_digit(sh.total, need);
+        prefix |= static_cast<uint32_t>(pick.digit) << shift;
+        need = pick.wanted;
+        if (need == pick.has) {
           prefix -= 1;
           need = 0;
           break;

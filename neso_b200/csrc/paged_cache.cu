@@ -73,17 +73,20 @@ __device__ __forceinline__ void store_vec(uint16_t* p, const Vec<N>& r) {
   }
 }
 
-constexpr int kRopeThreads = 256;
-constexpr int kRopeBatch = 3;    // items whose loads a thread has in flight
-constexpr int kRopeTokens = 4;   // tokens per CTA when there are many
+constexpr int kRopeTokens = 2;   // tokens per CTA when there are many
 constexpr int kMaxRopeDim = 1024;
 
+// kThreads per CTA, kBatch items requested at a time by each. Many tokens run
+// fastest in small CTAs with few registers (8192 tokens of 48 heads x 128: 128
+// threads, 2 items, 2 tokens 37.2 us; 256, 3, 4 41.7; 128, 3, 2 38.7; 64, 3, 1
+// 38.7), few tokens with a CTA for each that requests all its items at once (187 tokens: 256
+// threads, 3 items 4.4 us; 128, 2 5.0).
 // A CTA takes p.group tokens. Every head of q, k and v is D / (2 kVec) items
 // of two vectors: a rotated pair, or two that are copied (the rest of a
 // rotated head, and values). The first items are requested before the chain
 // position -> angles, which is walked once per CTA into shared memory.
-template <bool kBf16, int kVec>
-__global__ void __launch_bounds__(kRopeThreads) rope_paged_append_kernel(const __grid_constant__ RopeParams p) {
+template <bool kBf16, int kVec, int kThreads, int kBatch>
+__global__ void __launch_bounds__(kThreads) rope_paged_append_kernel(const __grid_constant__ RopeParams p) {
   extern __shared__ __align__(16) float angles[];  // [group][2][half]
   __shared__ int64_t places[kRopeTokens][2];        // element offsets in k_cache and v_cache, or -1
   const int tid = threadIdx.x;
@@ -117,11 +120,11 @@ __global__ void __launch_bounds__(kRopeThreads) rope_paged_append_kernel(const _
     if (it.h < rotated) return p.k + n * p.k_sn + (it.h - p.hq) * p.k_sh + it.d;
     return p.v + n * p.v_sn + (it.h - rotated) * p.v_sh + it.d;
   };
-  Vec<kVec> x[kRopeBatch], y[kRopeBatch];
+  Vec<kVec> x[kBatch], y[kBatch];
   auto request = [&](int i0) {
 #pragma unroll
-    for (int j = 0; j < kRopeBatch; ++j) {
-      const int i = i0 + j * kRopeThreads;
+    for (int j = 0; j < kBatch; ++j) {
+      const int i = i0 + j * kThreads;
       if (i < items) {
         const Item it = item_at(i);
         const uint16_t* src = source(it);
@@ -145,7 +148,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_paged_append_kernel(const _
     places[tid][0] = ko;
     places[tid][1] = vo;
   }
-  for (int i = tid; i < tokens * p.half; i += kRopeThreads) {
+  for (int i = tid; i < tokens * p.half; i += kThreads) {
     const int n = i / p.half, d = i - n * p.half;
     int axis = 0;
     while (axis < p.axes - 1 && d >= p.section_end[axis]) ++axis;
@@ -157,11 +160,11 @@ __global__ void __launch_bounds__(kRopeThreads) rope_paged_append_kernel(const _
   }
   __syncthreads();
 
-  for (int i0 = tid; i0 < items; i0 += kRopeBatch * kRopeThreads) {
+  for (int i0 = tid; i0 < items; i0 += kBatch * kThreads) {
     if (i0 != tid) request(i0);
 #pragma unroll
-    for (int j = 0; j < kRopeBatch; ++j) {
-      const int i = i0 + j * kRopeThreads;
+    for (int j = 0; j < kBatch; ++j) {
+      const int i = i0 + j * kThreads;
       if (i >= items) break;
       const Item it = item_at(i);
       const int64_t ko = places[it.n][0], vo = places[it.n][1];
@@ -195,12 +198,13 @@ __global__ void __launch_bounds__(kRopeThreads) rope_paged_append_kernel(const _
 
 template <bool kBf16, int kVec>
 int launch_rope(RopeParams p, cudaStream_t stream) {
-  // A token to a CTA while that leaves SMs idle, for the shorter latency.
-  p.group = p.N >= 8 * sm_count() ? kRopeTokens : 1;
+  const bool many = p.N >= 8 * sm_count();
+  p.group = many ? kRopeTokens : 1;
   p.per_head = page_divisor(static_cast<uint32_t>(p.D / (2 * kVec)));
   const unsigned grid = static_cast<unsigned>((p.N + p.group - 1) / p.group);
   const size_t smem = static_cast<size_t>(p.group) * 2 * p.half * sizeof(float);
-  cudaError_t e = launch_pdl(rope_paged_append_kernel<kBf16, kVec>, dim3(grid), dim3(kRopeThreads), smem, stream, p);
+  cudaError_t e = many ? launch_pdl(rope_paged_append_kernel<kBf16, kVec, 128, 2>, dim3(grid), dim3(128), smem, stream, p)
+                       : launch_pdl(rope_paged_append_kernel<kBf16, kVec, 256, 3>, dim3(grid), dim3(256), smem, stream, p);
   return e == cudaSuccess ? ok() : cuda_fail(e, "rope_paged_append launch");
 }
 

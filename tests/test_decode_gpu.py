@@ -329,6 +329,7 @@ def test_attention_refusals(dev):
     (5, 1, 1, 80, 24, None, 1),
     (2, 1, 1, 64, 0, None, 16),            # nothing is rotated
     (300, 8, 8, 64, 32, None, 16),
+    (1201, 1, 1, 16, 8, [3, 5], 16),       # tokens enough for several to a CTA, the last alone
 ])
 def test_append(dev, N, hq, hkv, D, half, sections, page, dtype):
     g = _gen(N + D)

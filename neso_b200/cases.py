@@ -6,6 +6,10 @@
     python -m neso_b200.cases w8a16 --M 1 --N 11008 --K 4096
     python -m neso_b200.cases w4a16 --M 2048 --N 11008 --K 4096
     python -m neso_b200.cases vector_add --n 268435456
+    python -m neso_b200.cases paged_attention --B 64 --H 64 --Hkv 8 --S 4096 --D 128 [--page 16] [--weights]
+    python -m neso_b200.cases rope_append --N 8192 --H 32 --Hkv 8 --D 128
+    python -m neso_b200.cases kv_evict --B 8 --Hkv 8 --S 4096 --D 128 --budget 2048
+    python -m neso_b200.cases logits --B 128 --V 32000 --S 1024       (S: tokens of history)
 
 Each case launches the op ``--warmup`` times, then ``--iters`` times between
 CUDA events on the current stream, and prints one JSON line with the mean
@@ -76,7 +80,8 @@ def _time_graph(fn, warmup: int, iters: int) -> float:
 
 def main() -> None:
     ap = argparse.ArgumentParser()
-    ap.add_argument("case", choices=["fa2", "relpos", "gemm", "w8a16", "w4a16", "vector_add", "scale"])
+    ap.add_argument("case", choices=["fa2", "relpos", "gemm", "w8a16", "w4a16", "vector_add", "scale", "paged_attention",
+                                     "rope_append", "kv_evict", "logits"])
     ap.add_argument("--B", type=int, default=16)
     ap.add_argument("--H", type=int, default=16)
     ap.add_argument("--S", type=int, default=2048)
@@ -87,6 +92,11 @@ def main() -> None:
     ap.add_argument("--N", type=int, default=4096)
     ap.add_argument("--K", type=int, default=4096)
     ap.add_argument("--n", type=int, default=1 << 28)
+    ap.add_argument("--Hkv", type=int, default=8, help="kv heads of the paged cache")
+    ap.add_argument("--page", type=int, default=16, help="tokens per page")
+    ap.add_argument("--budget", type=int, default=1024, help="tokens that kv_evict keeps")
+    ap.add_argument("--V", type=int, default=32000, help="vocabulary of the logits")
+    ap.add_argument("--weights", action="store_true", help="paged attention that accumulates the softmax weights")
     ap.add_argument("--warmup", type=int, default=3)
     ap.add_argument("--iters", type=int, default=5)
     ap.add_argument("--graph", action="store_true",
@@ -146,6 +156,54 @@ def main() -> None:
             wbytes = a.K * a.N // 2
         res.update(shape=[a.M, a.N, a.K], us=t * 1e6, tflops=2.0 * a.M * a.N * a.K / t / 1e12,
                    weight_gbs=wbytes / t / 1e9)
+    elif a.case in ("paged_attention", "kv_evict"):
+        width = -(-a.S // a.page)
+        moved = 4 * a.Hkv * a.D * a.B
+        copies = _copies(moved * (a.S if a.case == "paged_attention" else 2 * a.budget))
+        caches = [tuple(torch.randn(2 * a.B * width, a.Hkv, a.page, a.D, device=dev, generator=g).half() for _ in range(2))
+                  for _ in range(copies)]
+        pages = torch.randperm(2 * a.B * width, device=dev, generator=g).to(torch.int32).view(2, a.B, width)
+        lens = torch.full((a.B,), a.S, dtype=torch.int32, device=dev)
+        w = torch.rand(a.B, a.Hkv, width * a.page, device=dev, generator=g)
+        w_out = torch.empty_like(w)
+        if a.case == "paged_attention":
+            q = torch.randn(a.B, a.H, a.D, device=dev, generator=g).half()
+            o = torch.empty_like(q)
+            kw = dict(weights=w, weights_out=w_out) if a.weights else {}
+            t = _time(lambda i: ops.paged_attention(q, *caches[i % copies], pages[0], lens, out=o, **kw), a.warmup, a.iters)
+            nbytes = moved * a.S + (8 * a.B * a.Hkv * a.S if a.weights else 0)
+            res.update(shape=[a.B, a.H, a.Hkv, a.S, a.D], weights=a.weights, us=t * 1e6, gbs=nbytes / t / 1e9)
+        else:
+            t = _time(lambda i: ops.kv_evict(*caches[i % copies], pages[0], lens, w, a.budget, a.budget // 8,
+                                             out_tables=pages[1], weights_out=w_out), a.warmup, a.iters)
+            nbytes = 2 * moved * min(a.budget, a.S) + 8 * a.B * a.Hkv * a.S
+            res.update(shape=[a.B, a.Hkv, a.S, a.D], budget=a.budget, us=t * 1e6, gbs=nbytes / t / 1e9)
+    elif a.case == "rope_append":
+        heads = a.H + 2 * a.Hkv
+        copies = _copies(4 * a.N * heads * a.D)
+        qkv = [torch.randn(a.N, heads, a.D, device=dev, generator=g).half() for _ in range(copies)]
+        angle = torch.rand(4096, a.D // 2, device=dev, generator=g) * 6.28
+        cos, sin = angle.cos(), angle.sin()
+        pages = -(-a.N // a.page)
+        kc, vc = (torch.empty(pages, a.Hkv, a.page, a.D, dtype=torch.float16, device=dev) for _ in range(2))
+        slots = torch.randperm(pages * a.page, device=dev, generator=g)[:a.N]
+        pos = torch.randint(0, 4096, (a.N,), device=dev, generator=g, dtype=torch.int32)
+        o = torch.empty(a.N, a.H, a.D, dtype=torch.float16, device=dev)
+        t = _time(lambda i: ops.rope_paged_append(qkv[i % copies][:, :a.H], qkv[i % copies][:, a.H:a.H + a.Hkv],
+                                                  qkv[i % copies][:, a.H + a.Hkv:], cos, sin, pos, slots, kc, vc, out=o),
+                  a.warmup, a.iters)
+        res.update(shape=[a.N, a.H, a.Hkv, a.D], us=t * 1e6, gbs=4 * a.N * heads * a.D / t / 1e9)
+    elif a.case == "logits":
+        copies = _copies(8 * a.B * a.V)
+        xs = [torch.randn(a.B, a.V, device=dev, generator=g) for _ in range(copies)]
+        history = torch.randint(0, a.V, (a.B, a.S), device=dev, generator=g, dtype=torch.int32)
+        lens = torch.full((a.B,), a.S, dtype=torch.int32, device=dev)
+        ones, repetition = torch.ones(a.B, device=dev), torch.full((a.B,), 1.1, device=dev)
+        mask = torch.full((a.B, -(-a.V // 32)), 0x55555555, dtype=torch.int32, device=dev)
+        y = torch.empty(a.B, a.V, device=dev)
+        t = _time(lambda i: ops.process_logits(xs[i % copies], history=history, history_lens=lens, repetition=repetition,
+                                               presence=ones, mask=mask, out=y), a.warmup, a.iters)
+        res.update(shape=[a.B, a.V], history=a.S, us=t * 1e6, gbs=8 * a.B * a.V / t / 1e9)
     else:
         x = torch.rand(a.n, device=dev, generator=g) * 2 - 1
         y = torch.rand(a.n, device=dev, generator=g) * 2 - 1

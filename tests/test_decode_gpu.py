@@ -673,6 +673,39 @@ def test_logits_refusals(dev):
         ops.process_logits(big[:, :100], out=big[:, 1:101])
 
 
+# ------------------------------------------------------ torch operators ----
+def test_torch_operators_match_tensor_api(dev):
+    import neso_b200.torch_ops  # noqa: F401
+    neso = torch.ops.neso
+    q, k, v, table, n, g = _setup(31, torch.float16, [90, 20], 4, 2, 64, 16)
+    table, n = table.cuda(), n.cuda()
+    w = torch.rand(2, 2, table.shape[1] * 16, generator=g).cuda()
+    w1, w2 = w.clone(), w.clone()
+    a = neso.paged_attention(q, k, v, table, n, 0.125, 20.0, 30, None, w1)
+    assert torch.equal(a, ops.paged_attention(q, k, v, table, n, 0.125, softcap=20.0, window=30, weights=w2))
+    assert torch.equal(w1, w2) and not torch.equal(w1, w)
+    b = neso.paged_attention(q, k, v, table, n, 0.125, 0.0, 0, torch.zeros(4, device=dev), None)
+    assert b.shape == q.shape
+    x, kw = _logit_inputs(32, 2, 500, 40, torch.float16)
+    kw = {name: t.cuda() for name, t in kw.items()}
+    assert torch.equal(neso.process_logits(x.cuda(), *kw.values()), ops.process_logits(x.cuda(), **kw))
+    k1, v1, k2, v2 = k.clone(), v.clone(), k.clone(), v.clone()
+    new = torch.randn(2, 8, 64, generator=g).half().cuda()
+    ang = torch.rand(50, 32, generator=g).cuda()
+    pos, slots = torch.tensor([3, 4], dtype=torch.int32, device=dev), torch.tensor([5, 20], device=dev)
+    args = (new[:, :4], new[:, 4:6], new[:, 6:], ang, ang, pos, slots)
+    assert torch.equal(neso.rope_paged_append(*args, k1, v1, None), ops.rope_paged_append(*args, k2, v2))
+    torch.testing.assert_close(k1, k2, rtol=0, atol=0, equal_nan=True)
+    r1 = neso.kv_evict(k1, v1, table, n, w1, 24, 4, 2, None)
+    r2 = ops.kv_evict(k2, v2, table, n, w2, 24, 4, sink=2)
+    assert torch.equal(r1[0], r2[0]) and torch.equal(r1[1], r2[1]) and torch.equal(w1, w2)
+    torch.testing.assert_close(v1, v2, rtol=0, atol=0, equal_nan=True)
+    for op, args in ((neso.paged_attention.default, (q, k1, v1, table, n, 0.1, 0.0, 0, None, w1)),
+                     (neso.kv_evict.default, (k1, v1, table, n, w1, 24, 4, 2, None)),
+                     (neso.process_logits.default, (x.cuda(), *kw.values()))):
+        torch.library.opcheck(op, args, test_utils=("test_schema", "test_faketensor"))
+
+
 # ------------------------------------------------------------- together ----
 def test_decoding_steps_together(dev):
     """Prompt, a few decoding steps, an eviction, more steps: the cache, the

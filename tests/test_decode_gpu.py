@@ -594,6 +594,45 @@ def test_logits(dev, B, V, T, dtype):
     _check_logits(x, kw)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,V,T,in_place", [(130, 16390, 200, False), (130, 16390, 200, True), (70, 33000, 17000, False),
+                                            (70, 33000, 17000, True), (64, 32769, 9000, False)])
+def test_logits_many_rows(dev, B, V, T, in_place, dtype):
+    # rows enough for the long slices, histories of several rounds, other alignments and in place
+    x, kw = _logit_inputs(V + T, B, V, T, dtype)
+    kw["history"] = torch.randint(0, V, (B, T), generator=_gen(T), dtype=torch.int32)
+    kw["mask"][::3], kw["mask"][1] = -1, 0
+    rows = torch.tensor([0, 1, 2, B // 2, B - 1])  # rows are independent: a few are worked out in 64 bits
+    wide = torch.zeros(B, V + 5, dtype=dtype, device=dev)
+    wide[:, 3:3 + V] = x.cuda()
+    xd = wide[:, 3:3 + V]
+    d = {k: v.cuda() for k, v in kw.items()}
+    got = ops.process_logits(xd, out=xd if in_place else None, **d)
+    if in_place:
+        assert bool((wide[:, :3] == 0).all()) and bool((wide[:, 3 + V:] == 0).all())
+    want, mag = oracle.decode_logits(x[rows], **{k: v[rows] for k, v in kw.items()})
+    g = got[rows.cuda()].cpu().double()
+    fin = want.isfinite()
+    torch.testing.assert_close(g[~fin], want[~fin], rtol=0, atol=0)
+    tol = (5 + 5) * U * mag + torch.finfo(dtype).eps / 2 * want.abs()
+    assert bool(((g - want).abs() <= tol)[fin].all())
+    again = x.cuda()
+    assert torch.equal(ops.process_logits(again, **d), got)  # other alignment, same values
+
+
+def test_logits_many_rows_parts(dev):
+    x, kw = _logit_inputs(77, 130, 16400, 60, torch.float32)
+    rows = torch.tensor([0, 77, 129])
+    for names in ((), ("mask",), ("bias_ids", "bias"), ("history", "history_lens", "prompt_lens", "presence", "repetition")):
+        part = {k: v for k, v in kw.items() if k in names}
+        want, mag = oracle.decode_logits(x[rows], **{k: v[rows] for k, v in part.items()})
+        for xd in (x.cuda(), x.cuda()):
+            got = ops.process_logits(xd, out=xd if names else None, **{k: v.cuda() for k, v in part.items()})
+            g = got[rows.cuda()].cpu().double()
+            fin = want.isfinite()
+            assert torch.equal(g[~fin], want[~fin]) and bool(((g - want).abs() <= 11 * U * mag)[fin].all())
+
+
 @pytest.mark.parametrize("names", [(), ("mask",), ("bias_ids", "bias"), ("history", "history_lens", "repetition"),
                                    ("history", "history_lens", "frequency"),
                                    ("history", "history_lens", "prompt_lens", "presence")])

@@ -9,6 +9,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ATen.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
 #include <cmath>
@@ -190,6 +191,7 @@ neso_stream_t stream_on(c10::Device device) {
 
 PyObject* rope_paged_append(PyObject* const* a) {
   const c10::Device device = device_of(a[0], "q");
+  const c10::cuda::CUDAGuard guard(device);  // the caller's device is back on return
   const at::Tensor& q = cuda_tensor(a[0], "q", {at::kHalf, at::kBFloat16}, 3, device);
   const Caches c = caches(a[7], a[8], device);
   const int64_t N = q.size(0), hq = q.size(1);
@@ -233,7 +235,6 @@ PyObject* rope_paged_append(PyObject* const* a) {
     if (!ok) value_error("sections must have one width per axis (" + str(axes) + ")");
   }
   const at::Tensor& slots = vector(a[6], "slots", at::kLong, N, device);
-  if (slots.numel() > 1 && slots.stride(0) != 1) value_error("slots must be contiguous");
   written(c.k, "k_cache");
   written(c.v, "v_cache");
   at::Tensor out;
@@ -257,6 +258,7 @@ PyObject* rope_paged_append(PyObject* const* a) {
 
 PyObject* paged_attention(PyObject* const* a) {
   const c10::Device device = device_of(a[0], "q");
+  const c10::cuda::CUDAGuard guard(device);  // the caller's device is back on return
   const at::Tensor& q = cuda_tensor(a[0], "q", {at::kHalf, at::kBFloat16}, 3, device);
   rows(q, "q");
   const Caches c = caches(a[1], a[2], device);
@@ -313,6 +315,7 @@ PyObject* paged_attention(PyObject* const* a) {
 
 PyObject* kv_evict(PyObject* const* a) {
   const c10::Device device = device_of(a[0], "k_cache");
+  const c10::cuda::CUDAGuard guard(device);
   const Caches c = caches(a[0], a[1], device);
   const int64_t B = tensor(a[2], "block_tables").dim() == 2 ? tensor(a[2], "block_tables").size(0) : 0;
   const at::Tensor& tables = table(a[2], "block_tables", B, device);
@@ -351,6 +354,7 @@ PyObject* kv_evict(PyObject* const* a) {
 
 PyObject* process_logits(PyObject* const* a) {
   const c10::Device device = device_of(a[0], "logits");
+  const c10::cuda::CUDAGuard guard(device);
   const at::Tensor& x = cuda_tensor(a[0], "logits", {at::kFloat, at::kHalf, at::kBFloat16}, 2, device);
   rows(x, "logits");
   const int64_t B = x.size(0), V = x.size(1);

@@ -904,7 +904,7 @@ __device__ __forceinline__ void tile_stats(const AttnParams& p, const Split& sp,
 }
 
 template <bool kBf16, int D, int NT, bool kScores>
-__global__ void __launch_bounds__(kJoinThreads, 2) paged_attention_join_kernel(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(kJoinThreads, kScores ? 4 : 2) paged_attention_join_kernel(const __grid_constant__ AttnParams p) {
   __shared__ JoinShared sh;
   if (!kScores || blockIdx.x < p.join_ctas) {
     pdl_wait();
@@ -1099,7 +1099,9 @@ int neso_paged_attention(const void* q, const void* k_cache, const void* v_cache
   if (rc != NESO_OK) return rc;
   if (num_pages < 0) return fail(NESO_ERR_INVALID_ARG, "num_pages must be >= 0");
   if (window < 0) return fail(NESO_ERR_INVALID_ARG, "window must be >= 0 (0 = no window)");
-  if (!(softcap >= 0.f) || softcap > 1e30f) return fail(NESO_ERR_INVALID_ARG, "softcap must be >= 0 and finite");
+  if (!(softcap >= 0.f) || softcap > 1e30f || (softcap > 0.f && !(fabsf(scale / softcap) <= 1e30f))) {
+    return fail(NESO_ERR_INVALID_ARG, "softcap must be >= 0 and finite, and scale / softcap finite");
+  }
   if ((weights_in != nullptr) != (weights_out != nullptr)) {
     return fail(NESO_ERR_INVALID_ARG, "weights_in and weights_out come together");
   }

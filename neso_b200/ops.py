@@ -213,8 +213,9 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.T
     Returns the kept tokens' old indexes (int32 [B, Hkv, budget], -1 behind the
     last) and the new lengths (int32 [B]).
 
-    Pages of ``out_tables`` must be other than every page of block_tables,
-    unless the table is the same; no page may belong to two sequences."""
+    ``out_tables`` is block_tables itself (or a view of its first columns), or
+    names pages of which none occurs in block_tables: a copy of block_tables is
+    neither. No page may belong to two sequences."""
     return (_binding or _load_binding()).kv_evict(k_cache, v_cache, block_tables, seq_lens, weights, budget, recent, sink,
                                                 out_tables, weights_out)
 

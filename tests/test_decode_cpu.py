@@ -29,7 +29,7 @@ def _attention(**kw):
 
 @pytest.mark.parametrize("kw,code", [
     (dict(dtype=2), I), (dict(Hq=7), I), (dict(Hkv=0), I), (dict(D=96), U), (dict(page=0), I), (dict(B=-1), I),
-    (dict(window=-1), I), (dict(softcap=-0.5), I), (dict(softcap=math.nan), I), (dict(softcap=math.inf), I),
+    (dict(window=-1), I), (dict(softcap=-0.5), I), (dict(softcap=math.nan), I), (dict(softcap=math.inf), I), (dict(softcap=1e-38), I),
     (dict(win=P), I), (dict(wout=P), I), (dict(q=None), I), (dict(lens=None), I), (dict(out=None), I),
     (dict(tables=None), I), (dict(k=None), I), (dict(k=P + 8), M), (dict(ks=(2048, 1024, 60)), M), (dict(vs=(2044, 1024, 64)), M),
     (dict(ks=(-2048, 1024, 64)), I), (dict(q=P + 2), M), (dict(q_sh=63), M), (dict(out=P + 2), M), (dict(ws=None), I),

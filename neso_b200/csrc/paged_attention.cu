@@ -21,8 +21,8 @@
 // holds a whole (sequence, kv head) writes the output itself; a run's first
 // and last pieces leave their maximum, sum and unnormalised output in the
 // workspace, and a second kernel joins them. Where the tables are short and
-// the (sequence, kv head) pairs fit the SMs, a CTA takes one pair and joins its
-// warps' parts itself: one launch, and no search for the runs.
+// the (sequence, kv head) pairs few, a cluster of CTAs takes each pair and joins
+// its warps' parts itself: one launch, and no search for the runs.
 //
 // Products: the tokens are the M rows of mma.m16n8k16 and the query heads its
 // N columns (S^T = K Q^T, O^T = V^T P^T), so a group of up to 8 heads costs one
@@ -31,10 +31,14 @@
 // P goes into the second product as a 16-bit value plus the 16-bit remainder
 // (relative error 2^-16 for bf16, 2^-22 for fp16), so the output's own
 // rounding is what remains; the tensor cores are idle enough to do it twice.
+#include <cooperative_groups.h>
+
 #include "paged.h"
 
 namespace neso {
 namespace {
+
+namespace cg = cooperative_groups;
 
 constexpr int kUnit = 16;      // tokens per unit
 constexpr int kStages = 3;     // units in flight per warp
@@ -614,10 +618,33 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? 2 : 4)
   }
 }
 
-// One CTA per (sequence, kv head) of one tile, its units dealt to the warps in turn;
-// the warps' parts are joined in shared memory, in a fixed order.
+// A cluster of CTAs per (sequence, kv head) of one tile, its units dealt to the
+// warps of all of them in turn. Each CTA joins its warps' parts in its shared
+// memory, then the CTAs take the fragments in turn and join them across the
+// cluster, all in a fixed order.
 constexpr int kSegWarps = 8;
 constexpr int kSegThreads = kSegWarps * 32;
+constexpr int kMaxCluster = 8;
+
+// Statistics and fragment of some pieces, added up one after the other.
+struct Joined {
+  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  __device__ __forceinline__ void add(const float4& st, const float4& x) {
+    const float n0 = fmaxf(m0, st.x), n1 = fmaxf(m1, st.z);
+    const float a0 = ex2_approx(m0 - safe_max(n0)), a1 = ex2_approx(m1 - safe_max(n1));
+    const float b0 = ex2_approx(st.x - safe_max(n0)), b1 = ex2_approx(st.z - safe_max(n1));
+    l0 = fmaf(st.y, b0, l0 * a0);
+    l1 = fmaf(st.w, b1, l1 * a1);
+    o.x = fmaf(x.x, b0, o.x * a0);
+    o.y = fmaf(x.y, b1, o.y * a1);
+    o.z = fmaf(x.z, b0, o.z * a0);
+    o.w = fmaf(x.w, b1, o.w * a1);
+    m0 = n0;
+    m1 = n1;
+  }
+  __device__ __forceinline__ float4 stats() const { return make_float4(m0, l0, m1, l1); }
+};
 
 template <bool kBf16, int D, int NT, bool kBias, bool kScores>
 __global__ void __launch_bounds__(kSegThreads) paged_attention_segment_kernel(const __grid_constant__ AttnParams p) {
@@ -626,21 +653,26 @@ __global__ void __launch_bounds__(kSegThreads) paged_attention_segment_kernel(co
   static_assert(kFrags * 32 * sizeof(float4) <= W::kRing, "a warp's part fits its ring");
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ float4 stats[kSegWarps][NT][4];
+  __shared__ float4 cta_stats[NT][4];
+  __shared__ float4 cta_part[kFrags][32];
   __shared__ float2 final_stats[NT * 8];  // reference point, 1 / l
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ctas = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_launch_dependents();
   pdl_wait();
+  const int segment = blockIdx.x / ctas, step = ctas * kSegWarps;
   Cursor c;
-  c.b = blockIdx.x / p.hkv;
-  c.hx = blockIdx.x % p.hkv;
+  c.b = segment / p.hkv;
+  c.hx = segment % p.hkv;
   c.s = span_of(p, c.b);
-  c.u = c.s.u0 + warp;
-  const int n = (c.s.u1 - c.u + kSegWarps - 1) / kSegWarps;
+  c.u = c.s.u0 + warp * ctas + rank;
+  const int n = c.u < c.s.u1 ? (c.s.u1 - c.u + step - 1) / step : 0;
   Cursor ld = c;
   W my(p, smem_u32(smem) + warp * W::kRing);
   auto request = [&](int stage, bool any) {
     my.request(ld, stage, any);
-    ld.u += kSegWarps;
+    ld.u += step;
   };
 #pragma unroll
   for (int s = 0; s < kStages - 1; ++s) request(s, s < n);
@@ -651,7 +683,7 @@ __global__ void __launch_bounds__(kSegThreads) paged_attention_segment_kernel(co
     const int next = stage + kStages - 1;
     request(next >= kStages ? next - kStages : next, i + kStages - 1 < n);
     my.add(c, stage);
-    c.u += kSegWarps;
+    c.u += step;
     if (++stage == kStages) stage = 0;
   }
   my.close();
@@ -666,44 +698,52 @@ __global__ void __launch_bounds__(kSegThreads) paged_attention_segment_kernel(co
   }
   __syncthreads();
   uint16_t* head0 = p.out + (static_cast<int64_t>(c.b) * p.hq + my.h0) * D;
+  auto write = [&](const Joined& j, int frag) {
+    const float i0 = inv_sum(j.l0), i1 = inv_sum(j.l1);
+    const float t[4] = {j.o.x * i0, j.o.y * i1, j.o.z * i0, j.o.w * i1};
+    store_out_tile<kBf16>(p, t, head0, D, frag / (D / 16), frag % (D / 16), my.nrows);
+  };
   for (int frag = warp; frag < kFrags; frag += kSegWarps) {
-    const int nt = frag / (D / 16), dt = frag % (D / 16);
-    float m0 = -INFINITY, m1 = -INFINITY;
+    const int nt = frag / (D / 16);
+    Joined j;
 #pragma unroll
     for (int k = 0; k < kSegWarps; ++k) {
-      m0 = fmaxf(m0, stats[k][nt][lane & 3].x);
-      m1 = fmaxf(m1, stats[k][nt][lane & 3].z);
+      j.add(stats[k][nt][lane & 3], reinterpret_cast<const float4*>(smem + k * W::kRing)[frag * 32 + lane]);
     }
-    const float r0 = safe_max(m0), r1 = safe_max(m1);
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    float l0 = 0.f, l1 = 0.f;
-#pragma unroll
-    for (int k = 0; k < kSegWarps; ++k) {
-      const float4 st = stats[k][nt][lane & 3];
-      const float4 x = reinterpret_cast<const float4*>(smem + k * W::kRing)[frag * 32 + lane];
-      const float a0 = ex2_approx(st.x - r0), a1 = ex2_approx(st.z - r1);
-      l0 = fmaf(st.y, a0, l0);
-      l1 = fmaf(st.w, a1, l1);
-      o.x = fmaf(x.x, a0, o.x);
-      o.y = fmaf(x.y, a1, o.y);
-      o.z = fmaf(x.z, a0, o.z);
-      o.w = fmaf(x.w, a1, o.w);
+    if (ctas == 1) {
+      write(j, frag);
+    } else {
+      cta_part[frag][lane] = j.o;
     }
-    const float i0 = inv_sum(l0), i1 = inv_sum(l1);
-    const float t[4] = {o.x * i0, o.y * i1, o.z * i0, o.w * i1};
-    store_out_tile<kBf16>(p, t, head0, D, nt, dt, my.nrows);
-    if (kScores && dt == 0 && lane < 4) {
-      final_stats[nt * 8 + lane * 2] = make_float2(r0, i0);
-      final_stats[nt * 8 + lane * 2 + 1] = make_float2(r1, i1);
+    if (frag % (D / 16) == 0 && lane < 4) cta_stats[nt][lane] = j.stats();
+  }
+  if (ctas > 1) {
+    cluster.sync();  // also: the scores of every CTA are written
+    for (int frag = rank + warp * ctas; frag < kFrags; frag += step) {
+      const int nt = frag / (D / 16);
+      Joined j;
+#pragma unroll 4
+      for (int k = 0; k < ctas; ++k) {
+        j.add(cluster.map_shared_rank(&cta_stats[nt][lane & 3], k)[0], cluster.map_shared_rank(&cta_part[frag][lane], k)[0]);
+      }
+      write(j, frag);
     }
+  } else if (kScores) {
+    __syncthreads();
   }
   if constexpr (kScores) {
-    // All heads of the group are here.
+    if (warp < NT && lane < 4) {
+      const float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
+      Joined j;
+      for (int k = 0; k < ctas; ++k) j.add(ctas == 1 ? cta_stats[warp][lane] : cluster.map_shared_rank(&cta_stats[warp][lane], k)[0], none);
+      final_stats[warp * 8 + lane * 2] = make_float2(safe_max(j.m0), inv_sum(j.l0));
+      final_stats[warp * 8 + lane * 2 + 1] = make_float2(safe_max(j.m1), inv_sum(j.l1));
+    }
     __syncthreads();
     const float* in = p.win + c.b * p.win_sb + c.hx * p.win_sh;
     float* out = p.wout + c.b * p.wout_sb + c.hx * p.wout_sh;
     const float* scores = p.scores + (static_cast<int64_t>(c.b) * p.hq + my.h0) * p.score_stride;
-    for (int t = threadIdx.x; t < c.s.len; t += kSegThreads) {
+    for (int t = rank * kSegThreads + threadIdx.x; t < c.s.len; t += ctas * kSegThreads) {
       float w = in[t];
       if (t >= c.s.lo) {
 #pragma unroll 4
@@ -714,6 +754,7 @@ __global__ void __launch_bounds__(kSegThreads) paged_attention_segment_kernel(co
       out[t] = w;
     }
   }
+  if (ctas > 1) cluster.sync();  // nobody reads this CTA's shared memory any more
 }
 
 // The second kernel. CTAs below p.join_ctas join the pieces of split segments.
@@ -738,25 +779,6 @@ constexpr int kWeightHeads = 4;  // heads whose scores a thread has requested
 struct JoinShared {
   float4 acc[kJoinWarps][32];
   float4 sums[kJoinWarps][4];
-};
-
-// Statistics and fragment of some pieces, added up one after the other.
-struct Joined {
-  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  __device__ __forceinline__ void add(const float4& st, const float4& x) {
-    const float n0 = fmaxf(m0, st.x), n1 = fmaxf(m1, st.z);
-    const float a0 = ex2_approx(m0 - safe_max(n0)), a1 = ex2_approx(m1 - safe_max(n1));
-    const float b0 = ex2_approx(st.x - safe_max(n0)), b1 = ex2_approx(st.z - safe_max(n1));
-    l0 = fmaf(st.y, b0, l0 * a0);
-    l1 = fmaf(st.w, b1, l1 * a1);
-    o.x = fmaf(x.x, b0, o.x * a0);
-    o.y = fmaf(x.y, b1, o.y * a1);
-    o.z = fmaf(x.z, b0, o.z * a0);
-    o.w = fmaf(x.w, b1, o.w * a1);
-    m0 = n0;
-    m1 = n1;
-  }
 };
 
 template <int D, int NT>
@@ -971,16 +993,20 @@ __global__ void __launch_bounds__(kJoinThreads, kScores ? 4 : 2) paged_attention
   }
 }
 
-// A CTA per (sequence, kv head) where these fit the SMs and the tables hold at
-// most this many tokens: 16 heads x 129 tokens (D = 64) take 4.4 us that way
-// and 8.6 us through runs and join; with long tables the one CTA's units would
-// follow each other for longer than the join takes.
+// A cluster per (sequence, kv head) where the clusters fit the SMs and the
+// tables hold at most kSegTokens tokens per CTA. One sequence, 32 / 8 heads,
+// D = 128, 512 / 1024 / 2048 / 8192 tokens: 5.9 / 6.7 / 8.1 / 14.7 us so,
+// 10.2 / 11.7 / 10.5 / 15.8 us as runs; beyond, the few CTAs' share of the
+// bandwidth falls behind (8 pairs of up to 9000 tokens: 19.6 against 16.5 us).
 constexpr int kSegTokens = 1024;
+// A CTA is worth having for this many tokens.
+constexpr int kSegLeast = 128;
 
 struct Plan {
   int group, tiles, rows, nt, ctas, warps;
   int64_t capacity;
   bool by_segment;
+  int cluster;  // CTAs per segment then
   size_t partials, stats, splits, scores, head_stats, score_stride, bytes;
 };
 
@@ -1004,7 +1030,9 @@ int make_plan(int B, int hq, int hkv, int D, int width, int page_size, bool weig
   if (segments > INT32_MAX || units + segments * kStart > INT32_MAX) {
     return fail(NESO_ERR_UNSUPPORTED, "batch x heads x table width exceeds 2^31 units of %d tokens", kUnit);
   }
-  pl.by_segment = segments <= sm_count() && pl.capacity <= kSegTokens && pl.tiles == 1;
+  pl.cluster = 1;
+  while (pl.cluster < kMaxCluster && segments * pl.cluster * 2 <= sm_count() && pl.cluster * kSegLeast < pl.capacity) pl.cluster *= 2;
+  pl.by_segment = segments <= sm_count() && pl.capacity <= static_cast<int64_t>(pl.cluster) * kSegTokens && pl.tiles == 1;
   const int64_t full = static_cast<int64_t>(sm_count()) * (D == 128 ? 2 : 4);
   pl.ctas = static_cast<int>(units < full ? (units > 1 ? units : 1) : full);
   pl.warps = pl.ctas * kWarps;
@@ -1034,7 +1062,21 @@ int launch_attention(const AttnParams& p, const Plan& pl, cudaStream_t stream) {
     auto* kern = paged_attention_segment_kernel<kBf16, D, NT, kBias, kScores>;
     const int rc = kernel_setup(reinterpret_cast<const void*>(kern), smem, nullptr);
     if (rc != NESO_OK) return rc;
-    const cudaError_t e = launch_pdl(kern, dim3(p.B * p.hkv), dim3(kSegThreads), smem, stream, p);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(p.B * p.hkv * pl.cluster));
+    cfg.blockDim = dim3(kSegThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(pl.cluster);
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
     return e == cudaSuccess ? ok() : cuda_fail(e, "paged_attention launch");
   }
   constexpr int smem = kWarps * W::kRing;

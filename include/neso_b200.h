@@ -344,8 +344,8 @@ NESO_API int neso_paged_attention(const void* q, const void* k_cache, const void
                                   int64_t v_stride_head, int64_t v_stride_token, int32_t table_width,
                                   int64_t table_stride, int64_t win_stride_b, int64_t win_stride_h,
                                   int64_t wout_stride_b, int64_t wout_stride_h, neso_stream_t stream);
-/* Bytes of workspace that neso_paged_attention needs on the current device;
- * negative (a status code) for arguments that it would refuse. */
+/* Bytes of workspace that neso_paged_attention needs on the current device (0:
+ * none, workspace may be NULL); negative (a status code) for arguments that it would refuse. */
 NESO_API int64_t neso_paged_attention_workspace(int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int32_t table_width,
                                                 int32_t page_size, int32_t with_weights);
 

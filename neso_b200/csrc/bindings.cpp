@@ -9,6 +9,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -183,6 +184,12 @@ T* data_or_null(PyObject* o) {
   return o == Py_None ? nullptr : static_cast<T*>(THPVariable_Unpack(o).data_ptr());
 }
 
+// A new tensor, straight from the CUDA allocator on the current stream (through
+// the dispatcher it takes half a microsecond more).
+at::Tensor empty(at::IntArrayRef sizes, at::ScalarType type, c10::Device device) {
+  return at::Tensor(at::detail::empty_cuda(sizes, type, device, c10::nullopt));
+}
+
 neso_stream_t stream_on(c10::Device device) {
   const int rc = entry.set_device(device.index());
   if (rc != NESO_OK) throw rc;
@@ -239,7 +246,7 @@ PyObject* rope_paged_append(PyObject* const* a) {
   written(c.v, "v_cache");
   at::Tensor out;
   if (a[10] == Py_None) {
-    out = at::empty({N, hq, c.dim}, q.options());
+    out = empty({N, hq, c.dim}, q.scalar_type(), device);
   } else {
     out = cuda_tensor(a[10], "out", {q.scalar_type()}, 3, device);
     if (out.sizes() != q.sizes() || !out.is_contiguous()) value_error("out must be contiguous and of q's shape");
@@ -290,7 +297,7 @@ PyObject* paged_attention(PyObject* const* a) {
   }
   at::Tensor out;
   if (a[11] == Py_None) {
-    out = at::empty({B, hq, c.dim}, q.options());
+    out = empty({B, hq, c.dim}, q.scalar_type(), device);
   } else {
     out = cuda_tensor(a[11], "out", {q.scalar_type()}, 3, device);
     if (out.sizes() != q.sizes() || !out.is_contiguous()) value_error("out must be contiguous and of q's shape");
@@ -302,11 +309,12 @@ PyObject* paged_attention(PyObject* const* a) {
   if (need < 0) throw static_cast<int>(need);
   // A workspace of the call's own, from torch's allocator: calls on other
   // streams and captured graphs have theirs.
-  const at::Tensor workspace = at::empty({need}, q.options().dtype(at::kByte));
+  at::Tensor workspace;
+  if (need > 0) workspace = empty({need}, at::kByte, device);
   const int rc = entry.paged_attention(
       q.data_ptr(), c.k.data_ptr(), c.v.data_ptr(), data<int32_t>(tables), data<int32_t>(lens), data_or_null<float>(a[8]),
       weighted ? data_or_null<float>(a[9]) : nullptr, weighted ? data_or_null<float>(wout) : nullptr, out.data_ptr(),
-      workspace.data_ptr(), need, code_of(q.scalar_type()), b32, hq32, c.heads, c.dim, scale, softcap, window, step_of(q, 0),
+      need > 0 ? workspace.data_ptr() : nullptr, need, code_of(q.scalar_type()), b32, hq32, c.heads, c.dim, scale, softcap, window, step_of(q, 0),
       step_of(q, 1), c.pages, c.page_size, step_of(c.k, 0), step_of(c.k, 1), step_of(c.k, 2), step_of(c.v, 0), step_of(c.v, 1),
       step_of(c.v, 2), width, step_of(tables, 0), win_s[0], win_s[1], wout_s[0], wout_s[1], stream);
   if (rc != NESO_OK) throw rc;
@@ -333,9 +341,8 @@ PyObject* kv_evict(PyObject* const* a) {
   written(c.k, "k_cache");
   written(c.v, "v_cache");
   written(wo, "weights_out");
-  const auto ints = tables.options();
-  at::Tensor kept = at::empty({B, c.heads, budget > 0 ? budget : 0}, ints);
-  at::Tensor new_lens = at::empty({B}, ints);
+  at::Tensor kept = empty({B, c.heads, budget > 0 ? budget : 0}, at::kInt, device);
+  at::Tensor new_lens = empty({B}, at::kInt, device);
   const neso_stream_t stream = stream_on(device);
   const int rc = entry.kv_evict(
       c.k.data_ptr(), c.v.data_ptr(), data<int32_t>(tables), data<int32_t>(to), data<int32_t>(lens), data<float>(wi),
@@ -397,7 +404,7 @@ PyObject* process_logits(PyObject* const* a) {
   }
   at::Tensor out;
   if (a[10] == Py_None) {
-    out = at::empty({B, V}, x.options());
+    out = empty({B, V}, x.scalar_type(), device);
   } else {
     out = cuda_tensor(a[10], "out", {x.scalar_type()}, 2, device);
     rows(out, "out");

@@ -1037,11 +1037,14 @@ int make_plan(int B, int hq, int hkv, int D, int width, int page_size, bool weig
   pl.ctas = static_cast<int>(units < full ? (units > 1 ? units : 1) : full);
   pl.warps = pl.ctas * kWarps;
   pl.partials = 0;
-  size_t at = round_up(static_cast<size_t>(pl.warps) * 2 * pl.nt * (D / 16) * 32 * sizeof(float4));
-  pl.stats = at;
-  at += round_up(static_cast<size_t>(pl.warps) * 2 * pl.nt * 4 * sizeof(float4));
-  pl.splits = at;
-  at += round_up(static_cast<size_t>(pl.warps) * 2 * sizeof(Split));
+  size_t at = 0;
+  if (!pl.by_segment) {
+    at = round_up(static_cast<size_t>(pl.warps) * 2 * pl.nt * (D / 16) * 32 * sizeof(float4));
+    pl.stats = at;
+    at += round_up(static_cast<size_t>(pl.warps) * 2 * pl.nt * 4 * sizeof(float4));
+    pl.splits = at;
+    at += round_up(static_cast<size_t>(pl.warps) * 2 * sizeof(Split));
+  }
   if (weights) {
     pl.score_stride = static_cast<size_t>((pl.capacity + kUnit - 1) / kUnit * kUnit);
     pl.scores = at;
@@ -1164,7 +1167,7 @@ int neso_paged_attention(const void* q, const void* k_cache, const void* v_cache
       q_stride_h % 2 != 0) {
     return fail(NESO_ERR_MISALIGNED, "q, out and q's strides must be multiples of 4 bytes");
   }
-  if (workspace == nullptr || workspace_bytes < static_cast<int64_t>(pl.bytes)) {
+  if (pl.bytes > 0 && (workspace == nullptr || workspace_bytes < static_cast<int64_t>(pl.bytes))) {
     return fail(NESO_ERR_INVALID_ARG, "workspace holds %lld bytes, %lld are needed",
                 static_cast<long long>(workspace == nullptr ? 0 : workspace_bytes), static_cast<long long>(pl.bytes));
   }

@@ -32,8 +32,8 @@ def _attention(**kw):
     (dict(window=-1), I), (dict(softcap=-0.5), I), (dict(softcap=math.nan), I), (dict(softcap=math.inf), I), (dict(softcap=1e-38), I),
     (dict(win=P), I), (dict(wout=P), I), (dict(q=None), I), (dict(lens=None), I), (dict(out=None), I),
     (dict(tables=None), I), (dict(k=None), I), (dict(k=P + 8), M), (dict(ks=(2048, 1024, 60)), M), (dict(vs=(2044, 1024, 64)), M),
-    (dict(ks=(-2048, 1024, 64)), I), (dict(q=P + 2), M), (dict(q_sh=63), M), (dict(out=P + 2), M), (dict(ws=None), I),
-    (dict(ws_bytes=16), I), (dict(ws=P + 4), M), (dict(pages=-1), I),
+    (dict(ks=(-2048, 1024, 64)), I), (dict(q=P + 2), M), (dict(q_sh=63), M), (dict(out=P + 2), M), (dict(ws=None, width=4000), I),
+    (dict(ws_bytes=16, width=4000), I), (dict(ws=P + 4), M), (dict(pages=-1), I),
     (dict(B=1 << 16, Hq=1 << 10, Hkv=1 << 10, width=1 << 20), U),
     (dict(B=0), _lib.NESO_OK),
 ])
@@ -45,7 +45,8 @@ def test_attention_entry_refuses_before_the_device(kw, code):
 def test_attention_workspace():
     f = _lib.lib().neso_paged_attention_workspace
     assert f(2, 8, 3, 64, 4, 16, 0) == I and f(2, 8, 2, 96, 4, 16, 0) == U
-    assert 0 < f(2, 8, 2, 64, 4, 16, 0) < f(2, 8, 2, 64, 4, 16, 1)
+    assert 0 == f(2, 8, 2, 64, 4, 16, 0) < f(2, 8, 2, 64, 4, 16, 1)  # short tables: clusters join by themselves
+    assert 0 < f(2, 8, 2, 64, 4000, 16, 0) < f(2, 8, 2, 64, 4000, 16, 1)
     # scores of every query head and token of the table
     assert f(3, 8, 2, 64, 100, 16, 1) - f(3, 8, 2, 64, 100, 16, 0) >= 3 * 8 * 1600 * 4
 

@@ -31,6 +31,12 @@
 // P goes into the second product as a 16-bit value plus the 16-bit remainder
 // (relative error 2^-16 for bf16, 2^-22 for fp16), so the output's own
 // rounding is what remains; the tensor cores are idle enough to do it twice.
+//
+// Measured (B200, D = 128): one sequence of 131071 tokens, 32 / 8 heads, 93 us =
+// 5.8 TB/s of keys and values, 88 % of the rate of a large copy; 64 ragged
+// sequences of 5 to 8192 tokens, 64 / 8 heads, 74.5 us = 5.6 TB/s. What is
+// missing: 5 us until the first keys arrive, the join (4 us), and equal runs
+// that end between 82 and 98 us because SMs reach memory at different rates.
 #include <cooperative_groups.h>
 
 #include "paged.h"
@@ -44,8 +50,12 @@ constexpr int kUnit = 16;      // tokens per unit
 constexpr int kStages = 3;     // units in flight per warp
 constexpr int kWarps = 4;      // warps per CTA
 constexpr int kThreads = kWarps * 32;
-constexpr int kStart = 4;      // cost of starting a segment, in units
-constexpr int kMinRun = 4;     // least points of a run
+// Cost of starting a segment, in units (64 ragged sequences: 77.6 us; 86.7 with
+// 0, 76.5 with 2, 78.3 with 8).
+constexpr int kStart = 4;
+// Least points of a run: shorter ones leave more pieces to join, longer ones
+// fewer warps (2048 tokens as runs: 10.7 us with 2, 10.6 with 4, 14.3 with 6).
+constexpr int kMinRun = 4;
 constexpr float kLog2e = 1.4426950408889634f;
 
 // A segment that several runs share: its index (sequence, kv head, tile), its

@@ -8,13 +8,17 @@
 //
 // kv_evict, first kernel: for each (sequence, kv head) the kept set is found by
 // a radix selection on the weights' bits. Up to kShortLen tokens one CTA does
-// it in registers and shared memory; longer sequences are counted by a cluster
-// through its shared memory. Second kernel: the kept rows move together, in
-// order. Under a table of their own they move independently of each other. In
-// place, a cluster moves the rows of one (sequence, kv head) a step at a time:
-// row j comes from row src_j >= j, so when all rows of a step are in shared
-// memory (a cluster barrier), the rows that it overwrites are not the source
-// of any later step, and later steps may already be on their way in.
+// it in registers and shared memory (a cluster's common count costs two cluster
+// barriers a digit: 66 us for the case below when every length took it, 43.6
+// without); longer sequences are counted by a cluster through its shared memory.
+// Second kernel: the kept rows move together, in order. Under a table of their
+// own they move independently of each other. In place, a cluster moves the rows
+// of one (sequence, kv head) a step at a time: row j comes from row src_j >= j,
+// so when all rows of a step are in shared memory (a cluster barrier), the rows
+// that it overwrites are not the source of any later step, and later steps may
+// already be on their way in. 8 sequences x 8 heads of up to 4096 tokens to
+// 2048, D = 128: 34.5 us under a table of their own, of which the rows take 22.3
+// (6 TB/s read and written, as a plain copy) and the selection the rest.
 #include <cooperative_groups.h>
 
 #include "paged.h"

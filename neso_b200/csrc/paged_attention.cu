@@ -1003,8 +1003,10 @@ __global__ void __launch_bounds__(kJoinThreads, kScores ? 4 : 2) paged_attention
   }
 }
 
-// A cluster per (sequence, kv head) where the clusters fit the SMs and the
-// tables hold at most kSegTokens tokens per CTA. One sequence, 32 / 8 heads,
+// A cluster per (sequence, kv head) where the clusters fit the SMs (two CTAs each
+// at D = 64: 256 pairs of up to 300 tokens 7.0 us, as runs 11.6; at D = 128 one:
+// 160 pairs of 900 tokens 22.1 us so, 20.0 as runs) and the tables hold at most
+// kSegTokens tokens per CTA. One sequence, 32 / 8 heads,
 // D = 128, 512 / 1024 / 2048 / 8192 tokens: 5.9 / 6.7 / 8.1 / 14.7 us so,
 // 10.2 / 11.7 / 10.5 / 15.8 us as runs; beyond, the few CTAs' share of the
 // bandwidth falls behind (8 pairs of up to 9000 tokens: 19.6 against 16.5 us).
@@ -1042,7 +1044,7 @@ int make_plan(int B, int hq, int hkv, int D, int width, int page_size, bool weig
   }
   pl.cluster = 1;
   while (pl.cluster < kMaxCluster && segments * pl.cluster * 2 <= sm_count() && pl.cluster * kSegLeast < pl.capacity) pl.cluster *= 2;
-  pl.by_segment = segments <= sm_count() && pl.capacity <= static_cast<int64_t>(pl.cluster) * kSegTokens && pl.tiles == 1;
+  pl.by_segment = segments <= sm_count() * (D == 64 ? 2 : 1) && pl.capacity <= static_cast<int64_t>(pl.cluster) * kSegTokens && pl.tiles == 1;
   const int64_t full = static_cast<int64_t>(sm_count()) * (D == 128 ? 2 : 4);
   pl.ctas = static_cast<int>(units < full ? (units > 1 ? units : 1) : full);
   pl.warps = pl.ctas * kWarps;

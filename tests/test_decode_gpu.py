@@ -107,6 +107,7 @@ ATTENTION = [
     ([300] * 9, 24, 8, 64, 24),
     ([9000], 4, 1, 128, 64),
     ([60] * 40, 12, 4, 64, 16),
+    ([30, 70] * 40, 8, 4, 64, 16),     # more pairs than clusters take
 ]
 
 

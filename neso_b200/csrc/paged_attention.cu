@@ -635,6 +635,12 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? 2 : 4)
 constexpr int kSegWarps = 8;
 constexpr int kSegThreads = kSegWarps * 32;
 constexpr int kMaxCluster = 8;
+// Very few pairs: clusters of this size, which a GPC of the B200 still holds (a
+// CTA to an SM at D = 128, so that only half the SMs are counted on). One
+// sequence of 8192 tokens: 16 / 1 heads x 128 18.5 -> 12.9 us, 32 / 8 x 64
+// 12.2 -> 9.9; 32 / 8 x 128 would take 20.2 instead of 14.9, as the eight
+// clusters are not on the SMs together.
+constexpr int kBigCluster = 16;
 
 // Statistics and fragment of some pieces, added up one after the other.
 struct Joined {
@@ -1009,7 +1015,8 @@ __global__ void __launch_bounds__(kJoinThreads, kScores ? 4 : 2) paged_attention
 // kSegTokens tokens per CTA. One sequence, 32 / 8 heads,
 // D = 128, 512 / 1024 / 2048 / 8192 tokens: 5.9 / 6.7 / 8.1 / 14.7 us so,
 // 10.2 / 11.7 / 10.5 / 15.8 us as runs; beyond, the few CTAs' share of the
-// bandwidth falls behind (8 pairs of up to 9000 tokens: 19.6 against 16.5 us).
+// bandwidth falls behind (8 pairs of up to 9000 tokens: 19.6 against 16.5 us; at
+// D = 128 and 16 CTAs beyond half of that, 16384 tokens: 19.0 against 17.0).
 constexpr int kSegTokens = 1024;
 // A CTA is worth having for this many tokens.
 constexpr int kSegLeast = 128;
@@ -1044,7 +1051,11 @@ int make_plan(int B, int hq, int hkv, int D, int width, int page_size, bool weig
   }
   pl.cluster = 1;
   while (pl.cluster < kMaxCluster && segments * pl.cluster * 2 <= sm_count() && pl.cluster * kSegLeast < pl.capacity) pl.cluster *= 2;
-  pl.by_segment = segments <= sm_count() * (D == 64 ? 2 : 1) && pl.capacity <= static_cast<int64_t>(pl.cluster) * kSegTokens && pl.tiles == 1;
+  if (pl.cluster == kMaxCluster && pl.cluster * kSegLeast < pl.capacity && segments * kBigCluster * (D == 64 ? 1 : 2) <= sm_count()) {
+    pl.cluster = kBigCluster;
+  }
+  pl.by_segment = segments <= sm_count() * (D == 64 ? 2 : 1) && pl.tiles == 1 &&
+                  pl.capacity <= static_cast<int64_t>(pl.cluster) * (D == 128 && pl.cluster > kMaxCluster ? kSegTokens / 2 : kSegTokens);
   const int64_t full = static_cast<int64_t>(sm_count()) * (D == 128 ? 2 : 4);
   pl.ctas = static_cast<int>(units < full ? (units > 1 ? units : 1) : full);
   pl.warps = pl.ctas * kWarps;
@@ -1077,6 +1088,10 @@ int launch_attention(const AttnParams& p, const Plan& pl, cudaStream_t stream) {
     auto* kern = paged_attention_segment_kernel<kBf16, D, NT, kBias, kScores>;
     const int rc = kernel_setup(reinterpret_cast<const void*>(kern), smem, nullptr);
     if (rc != NESO_OK) return rc;
+    if (pl.cluster > kMaxCluster) {
+      const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute");
+    }
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(p.B * p.hkv * pl.cluster));
     cfg.blockDim = dim3(kSegThreads);

@@ -102,6 +102,8 @@ ATTENTION = [
     ([65, 300], 50, 1, 128, 32),       # group of fifty: four passes, the last short
     ([1000, 999, 998], 6, 2, 128, 128),
     ([0, 0], 4, 4, 64, 16),
+    ([8000], 3, 1, 64, 64),            # clusters of sixteen CTAs per pair
+    ([5000, 40], 32, 2, 128, 16),
     ([2000], 8, 2, 64, 16),            # clusters of eight, four and two CTAs per pair, and runs
     ([1500, 7, 0], 16, 4, 128, 16),
     ([300] * 9, 24, 8, 64, 24),
@@ -190,7 +192,7 @@ def test_attention_bad_pages_and_lengths(dev):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("hq,hkv,D,window,extra", [(4, 4, 64, 0, 2), (8, 1, 128, 0, 2), (20, 1, 64, 0, 2), (6, 2, 128, 40, 2),
-                                                   (8, 1, 128, 0, 700), (9, 1, 64, 40, 700)])  # extra: a table for runs
+                                                   (8, 1, 128, 0, 700), (9, 1, 64, 40, 700), (16, 1, 64, 0, 200)])  # extra: a table for runs
 def test_attention_weights(dev, hq, hkv, D, window, extra, dtype):
     lens = [0, 1, 31, 150, 700]
     q, k, v, table, n, g = _setup(hq, dtype, lens, hq, hkv, D, 16, extra_width=extra)

@@ -56,4 +56,18 @@ __device__ __forceinline__ uint32_t page_of(const PageDivisor& d, uint32_t token
   return static_cast<uint32_t>((hi + lo) >> d.shift);
 }
 
+// The two 16-bit types: pack with one rounding, unpack exactly.
+template <bool kBf16>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+  if (kBf16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  return pack_half2(lo, hi);
+}
+template <bool kBf16>
+__device__ __forceinline__ float2 unpack16(uint32_t x) {
+  if (kBf16) return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+  return __half22float2(*reinterpret_cast<const __half2*>(&x));
+}
 }  // namespace neso

@@ -4,7 +4,7 @@
 // and sums rounded separately, then once to 16 bits) and keys and values go to
 // their slots. One pass: every input byte is read once and every output byte
 // written once, so HBM bounds it (launch latency for a few tokens): 8192 tokens
-// of 32 + 8 + 8 heads x 128 in 37.4 us, 5.5 TB/s read and written.
+// of 32 + 8 + 8 heads x 128 in 37.0 us, 5.6 TB/s read and written.
 //
 // kv_evict, first kernel: for each (sequence, kv head) the kept set is found by
 // a radix selection on the weights' bits. Up to kShortLen tokens one CTA does
@@ -56,9 +56,17 @@ __device__ __forceinline__ uint16_t from_float(float x) {
 }
 
 template <int N>
-struct Vec {
+struct alignas(N == 8 ? 16 : 2) Vec {
   uint16_t e[N];
 };
+
+// Where the angle of pair d lies among `half` of them. Vectors of eight keep the
+// first fours of all columns, then the second ones, so that neighbouring lanes
+// read neighbouring float4.
+template <int kVec>
+__device__ __forceinline__ int angle_place(int d, int half) {
+  return kVec == 8 ? (d & 4) * (half >> 3) + (d >> 3) * 4 + (d & 3) : d;
+}
 template <int N>
 __device__ __forceinline__ Vec<N> load_vec(const uint16_t* p) {
   Vec<N> r;
@@ -159,9 +167,10 @@ __global__ void __launch_bounds__(kThreads) rope_paged_append_kernel(const __gri
     while (axis < p.axes - 1 && d >= p.section_end[axis]) ++axis;
     const int pos = p.positions[static_cast<int64_t>(axis) * p.N + n0 + n];
     const bool in = pos >= 0 && pos < p.table_rows;
-    const int64_t at = static_cast<int64_t>(pos) * p.half + d;
-    angles[(2 * n) * p.half + d] = in ? p.cos[at] : __int_as_float(0x7fc00000);
-    angles[(2 * n + 1) * p.half + d] = in ? p.sin[at] : __int_as_float(0x7fc00000);
+    const int64_t row = static_cast<int64_t>(pos) * p.half + d;
+    const int place = 2 * n * p.half + angle_place<kVec>(d, p.half);
+    angles[place] = in ? p.cos[row] : __int_as_float(0x7fc00000);
+    angles[place + p.half] = in ? p.sin[row] : __int_as_float(0x7fc00000);
   }
   __syncthreads();
 
@@ -171,7 +180,7 @@ __global__ void __launch_bounds__(kThreads) rope_paged_append_kernel(const __gri
     for (int j = 0; j < kBatch; ++j) {
       const int i = i0 + j * kThreads;
       if (i >= items) break;
-      const Item it = item_at(i);
+      const Item it = item_at(i);  // again: kept, it costs registers and 39.8 us
       const int64_t ko = places[it.n][0], vo = places[it.n][1];
       uint16_t* dst;
       if (it.h < p.hq) {
@@ -186,13 +195,28 @@ __global__ void __launch_bounds__(kThreads) rope_paged_append_kernel(const __gri
                              : static_cast<uint16_t*>(p.vc.base) + vo + (it.h - rotated) * p.vc.head_stride + it.d;
       }
       if (it.turned && ko >= 0) {
-        const float* cs = angles + 2 * it.n * p.half + it.d;
-        const float* sn = cs + p.half;
+        const float* cs = angles + 2 * it.n * p.half + angle_place<kVec>(it.d, p.half);
+        if (kVec == 8) {
+          uint32_t* xw = reinterpret_cast<uint32_t*>(&x[j]);
+          uint32_t* yw = reinterpret_cast<uint32_t*>(&y[j]);
 #pragma unroll
-        for (int e = 0; e < kVec; ++e) {
-          const float u = to_float<kBf16>(x[j].e[e]), w = to_float<kBf16>(y[j].e[e]);
-          x[j].e[e] = from_float<kBf16>(__fsub_rn(__fmul_rn(u, cs[e]), __fmul_rn(w, sn[e])));
-          y[j].e[e] = from_float<kBf16>(__fadd_rn(__fmul_rn(u, sn[e]), __fmul_rn(w, cs[e])));
+          for (int q4 = 0; q4 < 2; ++q4) {
+            const float4 c4 = *reinterpret_cast<const float4*>(cs + q4 * (p.half / 2));
+            const float4 s4 = *reinterpret_cast<const float4*>(cs + p.half + q4 * (p.half / 2));
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float2 u = unpack16<kBf16>(xw[2 * q4 + e]), w = unpack16<kBf16>(yw[2 * q4 + e]);
+              const float c0 = e ? c4.z : c4.x, c1 = e ? c4.w : c4.y, s0 = e ? s4.z : s4.x, s1 = e ? s4.w : s4.y;
+              xw[2 * q4 + e] = pack16<kBf16>(__fsub_rn(__fmul_rn(u.x, c0), __fmul_rn(w.x, s0)),
+                                             __fsub_rn(__fmul_rn(u.y, c1), __fmul_rn(w.y, s1)));
+              yw[2 * q4 + e] = pack16<kBf16>(__fadd_rn(__fmul_rn(u.x, s0), __fmul_rn(w.x, c0)),
+                                             __fadd_rn(__fmul_rn(u.y, s1), __fmul_rn(w.y, c1)));
+            }
+          }
+        } else {
+          const float u = to_float<kBf16>(x[j].e[0]), w = to_float<kBf16>(y[j].e[0]);
+          x[j].e[0] = from_float<kBf16>(__fsub_rn(__fmul_rn(u, cs[0]), __fmul_rn(w, cs[p.half])));
+          y[j].e[0] = from_float<kBf16>(__fadd_rn(__fmul_rn(u, cs[p.half]), __fmul_rn(w, cs[0])));
         }
       }
       store_vec<kVec>(dst, x[j]);

@@ -29,8 +29,9 @@
 // instruction per 16 x 16 block of the cache and ldmatrix reads each byte of
 // it once; groups up to 16 take two column tiles, larger ones several passes.
 // P goes into the second product as a 16-bit value plus the 16-bit remainder
-// (relative error 2^-16 for bf16, 2^-22 for fp16), so the output's own
-// rounding is what remains; the tensor cores are idle enough to do it twice.
+// (relative error 2^-16 for bf16; 2^-22 for fp16, and at most 2^-40 of the
+// row's largest weight, see kRaise), so the output's own rounding is what
+// remains; the tensor cores are idle enough to do it twice.
 //
 // Measured (B200, D = 128): one sequence of 131071 tokens, 32 / 8 heads, 93 us =
 // 5.8 TB/s of keys and values, 88 % of the rate of a large copy; 64 ragged
@@ -300,6 +301,10 @@ struct Warp {
   static constexpr int kChunks = kRowBytes / 16;   // 16-byte chunks per row
   static constexpr int kRowsPerCopy = 32 / kChunks;
   static constexpr int kCopies = kUnit / kRowsPerCopy;
+  // fp16 ends at 2^-24: of weights up to 1, the value and the remainder would both
+  // lose what lies below 2^-25, which the sum counts. Weights up to 2^kRaise keep
+  // 22 bits down to 2^-17 of the largest, and are off by 2^-40 of it below.
+  static constexpr float kRaise = kBf16 ? 0.f : 15.f;
 
   const AttnParams& p;
   const int lane;
@@ -460,8 +465,8 @@ struct Warp {
         const float ref = safe_max(mx);
         alpha[j] = ex2_approx(m[nt][j] - ref);
         m[nt][j] = mx;
-        s[nt][j] = ex2_approx(s[nt][j] - ref);
-        s[nt][2 + j] = ex2_approx(s[nt][2 + j] - ref);
+        s[nt][j] = ex2_approx((s[nt][j] - ref) + kRaise);
+        s[nt][2 + j] = ex2_approx((s[nt][2 + j] - ref) + kRaise);
         l[nt][j] = fmaf(l[nt][j], alpha[j], s[nt][j] + s[nt][2 + j]);
       }
       if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
@@ -498,14 +503,21 @@ struct Warp {
     }
   }
 
-  // The sums of the segment's weights, over the lanes.
+  // The sums of the segment's weights, over the lanes; weights count from 1 again.
   __device__ __forceinline__ void close() {
+    constexpr float kLower = kBf16 ? 1.f : 1.f / 32768.f;  // 2^-kRaise
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], d);
+        l[nt][j] *= kLower;
+      }
+#pragma unroll
+      for (int dt = 0; dt < D / 16; ++dt) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[nt][dt][e] *= kLower;
       }
     }
   }

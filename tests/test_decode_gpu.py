@@ -172,6 +172,41 @@ def test_attention_extreme_scores(dev):
     assert bool(got[0, 0].isnan().all()) and not bool(got[0, 1].isnan().any())
 
 
+def _uniform_pages(q, rows, values, dtype, dev):
+    """A cache whose page i holds one key and one value in every row: the first
+    element of the key is rows[i], every element of the value values[i]."""
+    hkv, D = q.shape[1], q.shape[2]
+    k = torch.zeros(len(rows), hkv, 16, D, dtype=dtype, device=dev)
+    v = torch.zeros_like(k)
+    for i, (x, y) in enumerate(zip(rows, values)):
+        k[i, :, :, 0], v[i] = x, y
+    return k, v
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B,hkv,D,n", [
+    (64, 8, 128, 8192),   # runs of thousands of tokens
+    (1, 3, 64, 8000),     # clusters
+    (40, 4, 64, 900),     # a CTA per pair
+])
+def test_attention_sink_and_flat_tail(dev, B, hkv, D, n, dtype):
+    # One token without a value 17.5 above the others (e^-17.5 = 2^-25.2): nearly
+    # all of the weight is its own, and the result is what the others add up to.
+    q = torch.zeros(B, 2 * hkv, D, dtype=dtype, device=dev)
+    q[:, ::2, 0], q[:, 1::2, 0] = 1.0, 0.984375
+    k, v = _uniform_pages(q[:, :hkv], [0.0, 0.0], [1.5, 1.5], dtype, dev)
+    k[1, :, 5, 0], v[1, :, 5] = 17.5, 0.0  # page 1 has the sink
+    table = torch.zeros(B, -(-n // 16), dtype=torch.int32, device=dev)
+    table[:, table.shape[1] // 3] = 1
+    got = ops.paged_attention(q, k, v, table, torch.full((B,), n, dtype=torch.int32, device=dev), scale=1.0)
+    for row, top in ((slice(0, None, 2), 17.5), (slice(1, None, 2), 17.5 * 0.984375)):
+        tail = (n - 1) * math.exp(-top)
+        want = 1.5 * tail / (1 + tail)
+        # sum p |v| is `want` itself; A = S = top, a sum of one product
+        tol = (2 * 2 * U * (1 + 8) * top + 2.0 ** -14) * want + torch.finfo(dtype).eps / 2 * want + 2.0 ** -25
+        assert float((got[:, row].double() - want).abs().max()) <= tol
+
+
 def test_attention_bad_pages_and_lengths(dev):
     # pages outside the cache are left out, lengths are clamped to the table
     q, k, v, table, n, _ = _setup(13, torch.float16, [100, 64, 50, 40], 4, 2, 64, 16)

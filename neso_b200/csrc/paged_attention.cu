@@ -302,9 +302,9 @@ struct Warp {
   static constexpr int kRowsPerCopy = 32 / kChunks;
   static constexpr int kCopies = kUnit / kRowsPerCopy;
   // fp16 ends at 2^-24: of weights up to 1, the value and the remainder would both
-  // lose what lies below 2^-25, which the sum counts. Weights up to 2^kRaise keep
+  // lose what lies below 2^-25, which the sum counts. Weights up to kRaise keep
   // 22 bits down to 2^-17 of the largest, and are off by 2^-40 of it below.
-  static constexpr float kRaise = kBf16 ? 0.f : 15.f;
+  static constexpr float kRaise = kBf16 ? 1.f : 32768.f;
 
   const AttnParams& p;
   const int lane;
@@ -465,8 +465,8 @@ struct Warp {
         const float ref = safe_max(mx);
         alpha[j] = ex2_approx(m[nt][j] - ref);
         m[nt][j] = mx;
-        s[nt][j] = ex2_approx((s[nt][j] - ref) + kRaise);
-        s[nt][2 + j] = ex2_approx((s[nt][2 + j] - ref) + kRaise);
+        s[nt][j] = ex2_approx(s[nt][j] - ref) * kRaise;  // an exact product
+        s[nt][2 + j] = ex2_approx(s[nt][2 + j] - ref) * kRaise;
         l[nt][j] = fmaf(l[nt][j], alpha[j], s[nt][j] + s[nt][2 + j]);
       }
       if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
@@ -505,7 +505,7 @@ struct Warp {
 
   // The sums of the segment's weights, over the lanes; weights count from 1 again.
   __device__ __forceinline__ void close() {
-    constexpr float kLower = kBf16 ? 1.f : 1.f / 32768.f;  // 2^-kRaise
+    constexpr float kLower = 1.f / kRaise;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll

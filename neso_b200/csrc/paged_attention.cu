@@ -28,10 +28,10 @@
 // N columns (S^T = K Q^T, O^T = V^T P^T), so a group of up to 8 heads costs one
 // instruction per 16 x 16 block of the cache and ldmatrix reads each byte of
 // it once; groups up to 16 take two column tiles, larger ones several passes.
-// P goes into the second product as a 16-bit value plus the 16-bit remainder
-// (relative error 2^-16 for bf16; 2^-22 for fp16, and at most 2^-40 of the
-// row's largest weight, see kRaise), so the output's own rounding is what
-// remains; the tensor cores are idle enough to do it twice.
+// P goes into the second product as a sum of 16-bit values, the next one the
+// remainder of those before (three in bf16: 2^-25 of the weight is left; two in
+// fp16: 2^-22, see kParts and kRaise), so the output's own rounding is what
+// remains; the tensor cores are idle enough to do it several times.
 //
 // Measured (B200, D = 128): one sequence of 131071 tokens, 32 / 8 heads, 93 us =
 // 5.8 TB/s of keys and values, 88 % of the rate of a large copy; 64 ragged
@@ -305,6 +305,11 @@ struct Warp {
   // lose what lies below 2^-25, which the sum counts. Weights up to kRaise keep
   // 22 bits down to 2^-17 of the largest, and are off by 2^-40 of it below.
   static constexpr float kRaise = kBf16 ? 1.f : 32768.f;
+  // Parts of a weight: 8 bits each in bf16, 11 in fp16. Two in bf16 leave 2^-17
+  // of the weight, more than the rest of the arithmetic (48 sequences of up to 1025
+  // visible tokens: results off by 1.0e-6 before their rounding, 4.0e-7 with three;
+  // 22.9 against 23.4 us).
+  static constexpr int kParts = kBf16 ? 3 : 2;
 
   const AttnParams& p;
   const int lane;
@@ -430,7 +435,7 @@ struct Warp {
       }
     }
     const bool v0 = (valid_bits >> (lane >> 2)) & 1, v1 = (valid_bits >> ((lane >> 2) + 8)) & 1;
-    uint32_t hi[NT][2], lo[NT][2];
+    uint32_t part[kParts][NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -480,10 +485,14 @@ struct Warp {
       }
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const uint32_t h = pack16<kBf16>(s[nt][2 * j], s[nt][2 * j + 1]);
-        const float2 f = unpack16<kBf16>(h);
-        hi[nt][j] = transpose8x8(h);
-        lo[nt][j] = transpose8x8(pack16<kBf16>(s[nt][2 * j] - f.x, s[nt][2 * j + 1] - f.y));
+        float2 rest = make_float2(s[nt][2 * j], s[nt][2 * j + 1]);
+#pragma unroll
+        for (int k = 0; k < kParts; ++k) {
+          const uint32_t h = pack16<kBf16>(rest.x, rest.y);
+          const float2 f = unpack16<kBf16>(h);
+          part[k][nt][j] = transpose8x8(h);
+          rest = make_float2(rest.x - f.x, rest.y - f.y);
+        }
       }
     }
     // O^T += V^T P^T: rows are d, read through transposing ldmatrix.
@@ -496,8 +505,8 @@ struct Warp {
         ldmatrix4_trans(rbase + (((dt * 2 + ((lane >> 3) & 1)) ^ (row & 7)) << 4), a);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          mma16816<kBf16>(o[nt][dt], a, hi[nt][0], hi[nt][1]);
-          mma16816<kBf16>(o[nt][dt], a, lo[nt][0], lo[nt][1]);
+#pragma unroll
+          for (int k = 0; k < kParts; ++k) mma16816<kBf16>(o[nt][dt], a, part[k][nt][0], part[k][nt][1]);
         }
       }
     }

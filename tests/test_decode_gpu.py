@@ -207,6 +207,35 @@ def test_attention_sink_and_flat_tail(dev, B, hkv, D, n, dtype):
         assert float((got[:, row].double() - want).abs().max()) <= tol
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D,page", [(64, 16), (128, 24)])
+def test_attention_differences_of_close_weights(dev, D, page, dtype):
+    # Values 1 and -1 of two tokens whose weights are nearly the same: the result
+    # is the weights' difference, and shows how exactly they were held.
+    B, hkv, n = 16, 4, 15
+    q, k, v, table, lens, g = _setup(D, dtype, [n] * B, 2 * hkv, hkv, D, page)
+    q[:] = 0
+    q[:, ::2, 0], q[:, 1::2, 0], q[:, :, 1] = 1.0, 0.8125, 2.0 ** -12
+    key, value = torch.zeros(B, hkv, n, D), torch.zeros(B, hkv, n, D)
+    coarse, fine = -torch.rand(B, hkv, 7, generator=g), -torch.rand(B, hkv, 14, generator=g)
+    key[:, :, 1::2, 0], key[:, :, 2::2, 0], key[:, :, 1:, 1] = coarse, coarse, fine
+    pair = torch.arange(D) % 7
+    value[:, :, 1 + 2 * pair, torch.arange(D)], value[:, :, 2 + 2 * pair, torch.arange(D)] = 1.0, -1.0
+    rows = table[:, 0].long().to(dev)
+    k[rows, :, :n], v[rows, :, :n] = key.to(dtype).to(dev), value.to(dtype).to(dev)
+    got = ops.paged_attention(q, k, v, table.to(dev), lens.to(dev), scale=1.0).cpu().double()
+    s = torch.einsum("bhgd,bhtd->bhgt", q.cpu().double().view(B, hkv, 2, D), key.to(dtype).double())
+    p = torch.exp(s)  # the first token's score is 0, the others' lie in [-1 - 2^-12, 0]
+    total = p.sum(-1, keepdim=True)
+    a, b = p[..., 1 + 2 * pair], p[..., 2 + 2 * pair]
+    want = ((a - b) / total).view(got.shape)
+    # A score of two products: one sum (2 U), its scale and its product (2 U); the
+    # exponential 2^-22 = 4 U; what the 16-bit parts leave, 4 U at most: 12 U of each
+    # weight, and 4 U for the truncated sum of the two. The total's error is relative.
+    tol = (28 * U * torch.maximum(a, b) / total).view(got.shape) + (torch.finfo(dtype).eps / 2 + 2.0 ** -16) * want.abs() + 2.0 ** -25
+    assert bool(((got - want).abs() <= tol).all()), float(((got - want).abs() / tol).max())
+
+
 def test_attention_bad_pages_and_lengths(dev):
     # pages outside the cache are left out, lengths are clamped to the table
     q, k, v, table, n, _ = _setup(13, torch.float16, [100, 64, 50, 40], 4, 2, 64, 16)

@@ -436,6 +436,7 @@ struct Warp {
     }
     const bool v0 = (valid_bits >> (lane >> 2)) & 1, v1 = (valid_bits >> ((lane >> 2) + 8)) & 1;
     uint32_t part[kParts][NT][2];
+    float alpha[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -460,7 +461,6 @@ struct Warp {
           }
         }
       }
-      float alpha[2];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         float mx = fmaxf(s[nt][j], s[nt][2 + j]);
@@ -468,20 +468,11 @@ struct Warp {
         for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
         mx = fmaxf(mx, m[nt][j]);
         const float ref = safe_max(mx);
-        alpha[j] = ex2_approx(m[nt][j] - ref);
+        alpha[nt][j] = ex2_approx(m[nt][j] - ref);
         m[nt][j] = mx;
         s[nt][j] = ex2_approx(s[nt][j] - ref) * kRaise;  // an exact product
         s[nt][2 + j] = ex2_approx(s[nt][2 + j] - ref) * kRaise;
-        l[nt][j] = fmaf(l[nt][j], alpha[j], s[nt][j] + s[nt][2 + j]);
-      }
-      if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
-#pragma unroll
-        for (int dt = 0; dt < D / 16; ++dt) {
-          o[nt][dt][0] *= alpha[0];
-          o[nt][dt][1] *= alpha[1];
-          o[nt][dt][2] *= alpha[0];
-          o[nt][dt][3] *= alpha[1];
-        }
+        l[nt][j] = fmaf(l[nt][j], alpha[nt][j], s[nt][j] + s[nt][2 + j]);
       }
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
@@ -495,7 +486,11 @@ struct Warp {
         }
       }
     }
-    // O^T += V^T P^T: rows are d, read through transposing ldmatrix.
+    // O^T = alpha O^T + V^T P^T: rows are d, read through transposing ldmatrix. The
+    // tensor cores cut each product off at the last bit of the sum they add to. A
+    // sum over all tokens would lose that much per token (32768 tokens of one sign in
+    // one run: 3e-4 of the result), so each unit's starts from zero, with the small
+    // parts, and an FMA adds it to the scaled output.
     {
       const int row = (lane & 7) + (lane >> 4) * 8;
       const uint32_t rbase = base + kHalf + row * kRowBytes;
@@ -505,8 +500,11 @@ struct Warp {
         ldmatrix4_trans(rbase + (((dt * 2 + ((lane >> 3) & 1)) ^ (row & 7)) << 4), a);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int k = 0; k < kParts; ++k) mma16816<kBf16>(o[nt][dt], a, part[k][nt][0], part[k][nt][1]);
+          for (int k = kParts - 1; k >= 0; --k) mma16816<kBf16>(sum, a, part[k][nt][0], part[k][nt][1]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[nt][dt][e] = fmaf(o[nt][dt][e], alpha[nt][e & 1], sum[e]);
         }
       }
     }

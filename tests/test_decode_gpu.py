@@ -236,6 +236,32 @@ def test_attention_differences_of_close_weights(dev, D, page, dtype):
     assert bool(((got - want).abs() <= tol).all()), float(((got - want).abs() / tol).max())
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D,hkv", [(64, 16), (128, 8)])
+def test_attention_long_sums(dev, D, hkv, dtype):
+    # Values 1 and 1 + eps, equal weights (others for each query head): the result lies a
+    # little above the middle between the two, so that a small loss on the way rounds it
+    # down. As many equal segments as the grid has warps: each works through whole ones.
+    units, B = 512, torch.cuda.get_device_properties(dev).multi_processor_count
+    eps = torch.finfo(dtype).eps
+    high = units // 2 + round(units * 4.6e-5 / eps)
+    q = torch.zeros(B, 4 * hkv, D, dtype=dtype, device=dev)
+    q[:, :, 0] = torch.linspace(0.5, 1.5, 4 * hkv)
+    k, v = _uniform_pages(q[:, :hkv], [-0.625] * 3, [1.0, 1.0 + eps, 1.0], dtype, dev)
+    k[2, :, 0, 0] = 0.0  # page 2 starts with the token that has the largest score
+    table = torch.zeros(B, units, dtype=torch.int32, device=dev)
+    table[:, torch.randperm(units - 1, generator=_gen(D))[:high].to(dev) + 1] = 1
+    table[:, 0] = 2
+    got = ops.paged_attention(q, k, v, table, torch.full((B,), 16 * units, dtype=torch.int32, device=dev), scale=1.0)
+    c = torch.exp(-0.625 * q[0, :, 0].double())
+    want = (1 + eps * 16 * high * c / (1 + (16 * units - 1) * c))[None, :, None]
+    # Output and total take one rounding per unit, at most U of a sum that rises evenly: U / 2
+    # of the whole per unit for each. Within a unit 16 products are cut off at 2 U of their
+    # sum, 32 U; 16 U for the sums over lanes, the quotient and the parts of a join.
+    tol = (units + 48) * U * want + eps / 2 * want
+    assert bool(((got.double() - want).abs() <= tol).all()), float(((got.double() - want).abs() / tol).max())
+
+
 def test_attention_bad_pages_and_lengths(dev):
     # pages outside the cache are left out, lengths are clamped to the table
     q, k, v, table, n, _ = _setup(13, torch.float16, [100, 64, 50, 40], 4, 2, 64, 16)

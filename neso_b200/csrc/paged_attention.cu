@@ -1190,7 +1190,9 @@ int neso_paged_attention(const void* q, const void* k_cache, const void* v_cache
   p.k = PagedCache{const_cast<void*>(k_cache), k_stride_page, k_stride_head, k_stride_token};
   p.v = PagedCache{const_cast<void*>(v_cache), v_stride_page, v_stride_head, v_stride_token};
   if (num_pages == 0) {
-    p.k.base = p.v.base = const_cast<void*>(q);  // nothing is read from it: no page is valid
+    // No page is valid and nothing is read, but copies of no bytes name an address all
+    // the same, and it has to lie on 16 bytes as any other (q need not).
+    p.k.base = p.v.base = reinterpret_cast<void*>(reinterpret_cast<uintptr_t>(q) & ~static_cast<uintptr_t>(15));
   } else {
     if ((rc = check_cache(p.k, "k_cache")) != NESO_OK) return rc;
     if ((rc = check_cache(p.v, "v_cache")) != NESO_OK) return rc;

@@ -280,6 +280,20 @@ def test_attention_bad_pages_and_lengths(dev):
     assert ops.paged_attention(q[:0], k, v, table[:0].cuda(), n[:0].cuda()).shape == (0, 4, 64)
 
 
+@pytest.mark.parametrize("page", [16, 24])
+@pytest.mark.parametrize("width", [3, 700])  # clusters, runs
+def test_attention_empty_cache_and_q_off_16_bytes(dev, width, page):
+    wide = torch.randn(2, 4, 66, generator=_gen(page)).half().to(dev)
+    q = wide[:, :, 2:]
+    empty = torch.empty(0, 2, page, 64, dtype=torch.float16, device=dev)
+    table = torch.zeros(2, width, dtype=torch.int32, device=dev)
+    n = torch.tensor([40, width * page], dtype=torch.int32, device=dev)
+    assert bool((ops.paged_attention(q, empty, empty, table, n) == 0).all())
+    w = torch.rand(2, 2, width * page, device=dev)
+    before = w.clone()
+    assert bool((ops.paged_attention(q, empty, empty, table, n, weights=w) == 0).all()) and torch.equal(w, before)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("hq,hkv,D,window,extra", [(4, 4, 64, 0, 2), (8, 1, 128, 0, 2), (20, 1, 64, 0, 2), (6, 2, 128, 40, 2),
                                                    (8, 1, 128, 0, 700), (9, 1, 64, 40, 700), (16, 1, 64, 0, 200)])  # extra: a table for runs

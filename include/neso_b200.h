@@ -349,7 +349,7 @@ NESO_API int neso_paged_attention(const void* q, const void* k_cache, const void
 NESO_API int64_t neso_paged_attention_workspace(int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int32_t table_width,
                                                 int32_t page_size, int32_t with_weights);
 
-/* Trim every sequence to at most `budget` tokens per kv head: the first
+/* Trim every sequence to at most `budget` (1 to 2^30) tokens per kv head: the first
  * `sink`, the last `recent` and, of those between, the ones with the largest
  * weight (ties: the lower index; NaN counts as largest) are kept, in order,
  * and moved to tokens 0, 1, ... under out_tables. kept [B, Hkv, budget] gets

@@ -331,6 +331,7 @@ PyObject* kv_evict(PyObject* const* a) {
   const int64_t tokens = tables.size(1) * c.page_size;
   const at::Tensor& wi = weights_of(a[4], "weights", B, c.heads, tokens, device);
   const int32_t budget = int_arg(a[5], "budget"), recent = int_arg(a[6], "recent"), sink = int_arg(a[7], "sink");
+  if (budget > (1 << 30)) value_error("budget is limited to 2^30 tokens (got " + str(budget) + ")");  // before `kept` is allocated
   const at::Tensor& to = a[8] == Py_None ? tables : table(a[8], "out_tables", B, device);
   const at::Tensor& wo = a[9] == Py_None ? wi : weights_of(a[9], "weights_out", B, c.heads, tokens, device);
   same_or_apart(wo, wi, "weights and weights_out");

@@ -255,6 +255,7 @@ struct EvictParams {
 // against 37.2 us for the whole eviction; 8 of 1023: 11.8 against 10.3).
 constexpr int kSmallTable = 2048;
 constexpr int kMaxCluster = 8;
+constexpr int kMostTokens = 1 << 30;
 constexpr int kDigitBits = 8;
 constexpr int kDigits = 1 << kDigitBits;
 constexpr int kCopiesOfHist = 8;   // counters of a digit, so that equal digits of a warp collide less
@@ -845,6 +846,8 @@ int neso_kv_evict(void* k_cache, void* v_cache, const int32_t* block_tables, con
   if (budget < 1 || recent < 0 || sink < 0 || static_cast<int64_t>(recent) + sink > budget) {
     return fail(NESO_ERR_INVALID_ARG, "need budget >= 1 and 0 <= recent + sink <= budget");
   }
+  // As for lengths: steps past the end of a row of `kept` stay in 32 bits.
+  if (budget > kMostTokens) return fail(NESO_ERR_UNSUPPORTED, "budget is limited to 2^30 tokens (got %d)", budget);
   if (static_cast<int64_t>(B) * Hkv * kMaxCluster > INT32_MAX) {
     return fail(NESO_ERR_UNSUPPORTED, "batch x heads is too large");
   }
@@ -881,9 +884,9 @@ int neso_kv_evict(void* k_cache, void* v_cache, const int32_t* block_tables, con
   p.recent = recent;
   p.sink = sink;
   p.num_pages = num_pages;
-  // Below 2^30, so that the kernel's steps past the end stay in 32 bits.
-  p.capacity = static_cast<int>(cap < (1 << 30) ? cap : (1 << 30));
-  p.out_capacity = static_cast<int>(ocap < (1 << 30) ? ocap : (1 << 30));
+  // At most 2^30, so that the kernel's steps past the end stay in 32 bits.
+  p.capacity = static_cast<int>(cap < kMostTokens ? cap : kMostTokens);
+  p.out_capacity = static_cast<int>(ocap < kMostTokens ? ocap : kMostTokens);
   p.page = page_divisor(static_cast<uint32_t>(page_size));
   const int64_t segments = static_cast<int64_t>(B) * Hkv;
   const int pieces = D / 8;

@@ -204,7 +204,7 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.T
              weights: torch.Tensor, budget: int, recent: int, sink: int = 0,
              out_tables: torch.Tensor | None = None,
              weights_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
-    """Trim every sequence to ``budget`` tokens per kv head: the first ``sink``,
+    """Trim every sequence to ``budget`` (1 to 2^30) tokens per kv head: the first ``sink``,
     the last ``recent`` and the ones with the largest ``weights`` (fp32 [B, Hkv,
     tokens], as ``paged_attention`` accumulates them) between. Kept tokens stay
     in order and move to the sequence's first slots under ``out_tables`` (int32

@@ -91,6 +91,12 @@ def test_evict_entry_refuses_before_the_device(kw, code):
     assert _evict(**kw) == code
 
 
+def test_evict_entry_refuses_budgets_that_steps_of_a_row_would_pass_32_bits_with():
+    assert _evict(budget=2 ** 31 - 1) == U and _evict(budget=2 ** 30 + 1) == U
+    assert "2^30" in _lib.last_error()
+    assert _evict(budget=2 ** 30, B=0) == _lib.NESO_OK
+
+
 def test_logits_entry_refuses_before_the_device():
     def f(x=P, out=P, dtype=2, B=2, V=100, hist=None, lens=None, T=0, ids=None, bias=None, n=0):
         return _lib.lib().neso_process_logits(x, out, dtype, B, V, V, V, hist, lens, None, T, T, None, None, None, ids, bias,

@@ -667,6 +667,13 @@ def test_evict_refusals(dev):
         ops.kv_evict(k, v, table, n, wide[:, :, :32], 8, 2, weights_out=wide[:, :, 4:36])
 
 
+def test_evict_refuses_a_budget_beyond_its_steps(dev):
+    q, k, v, table, n, _ = _setup(6, torch.float16, [30], 2, 2, 64, 16)
+    w = torch.zeros(1, 2, 32, device=dev)
+    with pytest.raises(ValueError, match="2\\^30"):  # refused before the 17 GB of `kept` are allocated
+        ops.kv_evict(k, v, table.cuda(), n.cuda(), w, 2 ** 31 - 1, 2)
+
+
 # --------------------------------------------------------------- logits ----
 def _logit_inputs(seed, B, V, T, dtype, n_bias=5):
     g = _gen(seed)

@@ -329,7 +329,8 @@ NESO_API int neso_rope_paged_append(const void* q, const void* k, const void* v,
  *   s = scale q.k;  s = softcap tanh(s / softcap) if softcap > 0;
  *   s += slopes[h] (t - (len - 1)) if slopes;  t > len - 1 - window if window > 0
  *   out [B, Hq, D] = softmax(s) v, in q's type.
- * With weights_in/weights_out (fp32 [B, Hkv, tokens], may be one buffer),
+ * With weights_in/weights_out (fp32 [B, Hkv, tokens], may be one buffer; tokens:
+ * at least the longest clamped length, only t < seq_lens[b] is touched),
  * weights_out[b, kv, t] = weights_in[b, kv, t] + the sum of the softmax
  * weights of the kv head's query heads, for t < seq_lens[b]; the rest is left.
  * A length is clamped to [0, table_width * page_size]; tokens of a page
@@ -355,8 +356,9 @@ NESO_API int64_t neso_paged_attention_workspace(int32_t B, int32_t Hq, int32_t H
  * and moved to tokens 0, 1, ... under out_tables. kept [B, Hkv, budget] gets
  * their old indexes (-1 behind the last), new_lens[b] = min(len, budget)
  * (a buffer other than seq_lens).
- * weights_out [B, Hkv, tokens] gets the kept weights and zero up to the old
- * length; it may be weights_in. out_tables may be the pointer block_tables (in
+ * Rows of weights_in hold table_width * page_size floats, whatever the lengths
+ * are: all of them may be read. weights_out gets the kept weights and zero up to
+ * the old length; it may be weights_in. out_tables may be the pointer block_tables (in
  * place); otherwise its pages have to be other than every page of
  * block_tables. Two sequences share no page. Kept tokens past the out table's end, and tokens
  * on a page outside [0, num_pages), are not moved. 16-bit elements; D a

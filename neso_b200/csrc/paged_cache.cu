@@ -846,6 +846,13 @@ int neso_kv_evict(void* k_cache, void* v_cache, const int32_t* block_tables, con
   if (budget < 1 || recent < 0 || sink < 0 || static_cast<int64_t>(recent) + sink > budget) {
     return fail(NESO_ERR_INVALID_ARG, "need budget >= 1 and 0 <= recent + sink <= budget");
   }
+  // The selection requests the weights of a whole table before it knows the length.
+  // Rows of a buffer that ends with the longest sequence are closer together.
+  const int64_t tokens = static_cast<int64_t>(table_width) * page_size;
+  if ((Hkv > 1 && win_stride_h > 0 && win_stride_h < tokens) || (B > 1 && win_stride_b > 0 && win_stride_b < tokens)) {
+    return fail(NESO_ERR_INVALID_ARG, "rows of weights_in must hold table_width * page_size = %lld tokens",
+                static_cast<long long>(tokens));
+  }
   // As for lengths: steps past the end of a row of `kept` stay in 32 bits.
   if (budget > kMostTokens) return fail(NESO_ERR_UNSUPPORTED, "budget is limited to 2^30 tokens (got %d)", budget);
   if (static_cast<int64_t>(B) * Hkv * kMaxCluster > INT32_MAX) {

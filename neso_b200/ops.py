@@ -206,7 +206,8 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.T
              weights_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """Trim every sequence to ``budget`` (1 to 2^30) tokens per kv head: the first ``sink``,
     the last ``recent`` and the ones with the largest ``weights`` (fp32 [B, Hkv,
-    tokens], as ``paged_attention`` accumulates them) between. Kept tokens stay
+    tokens], tokens at least width * page_size, as ``paged_attention``
+    accumulates them) between. Kept tokens stay
     in order and move to the sequence's first slots under ``out_tables`` (int32
     [B, width]; None: in place, under block_tables), their weights to the front
     of ``weights_out`` (None: in place), followed by zeros up to the old length.

@@ -97,6 +97,13 @@ def test_evict_entry_refuses_budgets_that_steps_of_a_row_would_pass_32_bits_with
     assert _evict(budget=2 ** 30, B=0) == _lib.NESO_OK
 
 
+def test_evict_entry_refuses_weights_that_end_before_the_table():
+    # three pages of 16 tokens: rows of 40 weights, in the batch or per kv head
+    assert _evict(w=(96, 40, 96, 48)) == I and "48 tokens" in _lib.last_error()
+    assert _evict(w=(40, 0, 96, 48)) == I
+    assert _evict(w=(80, 0, 96, 48), Hkv=1, B=0) == _evict(w=(0, 0, 96, 48), B=0) == _lib.NESO_OK
+
+
 def test_logits_entry_refuses_before_the_device():
     def f(x=P, out=P, dtype=2, B=2, V=100, hist=None, lens=None, T=0, ids=None, bias=None, n=0):
         return _lib.lib().neso_process_logits(x, out, dtype, B, V, V, V, hist, lens, None, T, T, None, None, None, ids, bias,

@@ -359,8 +359,9 @@ NESO_API int64_t neso_paged_attention_workspace(int32_t B, int32_t Hq, int32_t H
  * Rows of weights_in hold table_width * page_size floats, whatever the lengths
  * are: all of them may be read. weights_out gets the kept weights and zero up to
  * the old length; it may be weights_in. out_tables may be the pointer block_tables (in
- * place); otherwise its pages have to be other than every page of
- * block_tables. Two sequences share no page. Kept tokens past the out table's end, and tokens
+ * place). Otherwise each of its pages either lies where block_tables has it (a copy
+ * of the table, or one that keeps some pages: such a sequence moves in order, by one
+ * CTA per kv head) or does not occur in block_tables. Two sequences share no page. Kept tokens past the out table's end, and tokens
  * on a page outside [0, num_pages), are not moved. 16-bit elements; D a
  * multiple of 8, at most 256. */
 NESO_API int neso_kv_evict(void* k_cache, void* v_cache, const int32_t* block_tables, const int32_t* out_tables,

@@ -633,6 +633,43 @@ constexpr int kApartWarps = 8;
 constexpr int kApartRows = 16;
 constexpr int kApartLoads = 4;
 
+// A sequence whose out table names one of its pages at the page's old place (a copy
+// of the block table, or a table that keeps some pages) has rows that are a source
+// for one move and the end of another. One CTA moves all of them then, in order: the
+// rows of a step are all loaded before the first is stored, and later steps read
+// behind the rows that it stores.
+__device__ __forceinline__ void move_ordered(const EvictParams& p, int b, int h, int keep, const int32_t* kept) {
+  constexpr int kThreads = kApartWarps * 32;
+  const int pieces = p.D / 8, row_items = 2 * pieces;
+  const int rows = kThreads * kApartLoads / row_items;
+  for (int j0 = 0; j0 < keep; j0 += rows) {
+    uint4 x[kApartLoads];
+    uint16_t* dst[kApartLoads];
+#pragma unroll
+    for (int i = 0; i < kApartLoads; ++i) {
+      const int item = i * kThreads + threadIdx.x;
+      const int r = item / row_items, j = j0 + r;
+      dst[i] = nullptr;
+      if (r < rows && j < keep) {
+        const int2 from = place_of(p, p.tables + b * p.table_stride, kept[j]);
+        const int2 to = place_of(p, p.out_tables + b * p.out_stride, j);
+        if (from.x >= 0 && to.x >= 0) {
+          const int at = item - r * row_items;
+          const PagedCache& cache = at < pieces ? p.k : p.v;
+          uint16_t* head = static_cast<uint16_t*>(cache.base) + h * cache.head_stride + (at < pieces ? at : at - pieces) * 8;
+          x[i] = *reinterpret_cast<const uint4*>(head + from.x * cache.page_stride + from.y * cache.token_stride);
+          dst[i] = head + to.x * cache.page_stride + to.y * cache.token_stride;
+        }
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kApartLoads; ++i) {
+      if (dst[i] != nullptr) *reinterpret_cast<uint4*>(dst[i]) = x[i];
+    }
+  }
+}
+
 __global__ void __launch_bounds__(kApartWarps * 32) kv_move_apart_kernel(const __grid_constant__ EvictParams p) {
   const int seg = blockIdx.x;
   const int b = seg / p.hkv, h = seg % p.hkv;
@@ -640,8 +677,20 @@ __global__ void __launch_bounds__(kApartWarps * 32) kv_move_apart_kernel(const _
   const int keep = min(kept_tokens(p, b), p.out_capacity);
   const int32_t* kept = p.kept + (static_cast<int64_t>(b) * p.hkv + h) * p.budget;
   const int pieces = p.D / 8, row_items = 2 * pieces;
+  bool shared = false;  // a page of this sequence stays where it was
+  if (keep > 0) {
+    const int blocks = static_cast<int>(page_of(p.page, keep - 1)) + 1;
+    for (int i = threadIdx.x; i < blocks; i += kApartWarps * 32) {
+      shared = shared || p.tables[b * p.table_stride + i] == p.out_tables[b * p.out_stride + i];
+    }
+  }
+  shared = __syncthreads_or(shared);  // while the selection runs
   pdl_wait();
   pdl_launch_dependents();
+  if (shared) {
+    if (blockIdx.y == 0) move_ordered(p, b, h, keep, kept);
+    return;
+  }
   for (int j0 = (blockIdx.y * kApartWarps + warp) * kApartRows; j0 < keep; j0 += gridDim.y * kApartWarps * kApartRows) {
     const int mine = j0 + (lane & (kApartRows - 1));
     int2 place = make_int2(-1, 0);
@@ -927,7 +976,7 @@ int neso_kv_evict(void* k_cache, void* v_cache, const int32_t* block_tables, con
   cudaError_t e = launch(select, ctas, cap > kSmallTable ? 1024 : 512, kSelectBytes);
   if (e != cudaSuccess) return cuda_fail(e, "kv_evict select launch");
   const int64_t most = budget < cap ? budget : cap;
-  if (out_tables != block_tables) {
+  if (out_tables != block_tables || (B > 1 && out_stride != table_stride)) {
     const int64_t blocks = (most + kApartWarps * kApartRows - 1) / (kApartWarps * kApartRows);
     if (blocks == 0) return ok();
     e = launch_pdl(kv_move_apart_kernel, dim3(static_cast<unsigned>(segments), static_cast<unsigned>(blocks < 65535 ? blocks : 65535)),

@@ -214,9 +214,11 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.T
     Returns the kept tokens' old indexes (int32 [B, Hkv, budget], -1 behind the
     last) and the new lengths (int32 [B]).
 
-    ``out_tables`` is block_tables itself (or a view of its first columns), or
-    names pages of which none occurs in block_tables: a copy of block_tables is
-    neither. No page may belong to two sequences."""
+    ``out_tables`` is block_tables itself or a view of its first columns (in
+    place), or a table of its own whose pages either lie where block_tables has
+    them or do not occur in it. A sequence with pages that stay, as under a copy
+    of block_tables, moves in order and more slowly than in place. No page may
+    belong to two sequences."""
     return (_binding or _load_binding()).kv_evict(k_cache, v_cache, block_tables, seq_lens, weights, budget, recent, sink,
                                                 out_tables, weights_out)
 

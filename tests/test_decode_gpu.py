@@ -628,6 +628,43 @@ def test_evict_strided_cache_and_spare_table(dev):
     _check_evict(3, torch.float16, [90, 20], 2, 64, 16, 30, 8, 2, "apart", layout="joint", extra=4)
 
 
+@pytest.mark.parametrize("keeps", ["all pages", "some pages"])
+@pytest.mark.parametrize("lens,hkv,D,page,budget,recent,sink", [
+    ([0, 1, 5, 17], 2, 64, 4, 5, 2, 1),
+    ([333, 9], 3, 8, 24, 300, 100, 4),
+    ([50, 90], 2, 256, 16, 49, 0, 40),
+    ([300, 299], 2, 24, 1, 200, 3, 0),
+    ([4096, 4000, 3000, 50], 8, 128, 16, 2048, 256, 4),
+    ([9000], 1, 64, 64, 5000, 17, 3),
+])
+def test_evict_under_a_table_that_keeps_pages(dev, lens, hkv, D, page, budget, recent, sink, keeps):
+    q, k, v, table, n, g = _setup(len(lens) + D, torch.float16, lens, hkv, hkv, D, page, spare=sum(-(-x // page) for x in lens))
+    w = torch.rand(len(lens), hkv, table.shape[1] * page, generator=g).to(dev)
+    width = -(-min(budget, table.shape[1] * page) // page)
+    out = table[:, :width].clone()
+    if keeps == "some pages":
+        free = torch.tensor(sorted(set(range(k.shape[0])) - set(table[table >= 0].tolist())), dtype=torch.int32)
+        fresh = (torch.rand(out.shape, generator=g) < 0.5) & (out >= 0)
+        out[fresh] = free[:int(fresh.sum())]
+    k0, v0, w0 = k.clone(), v.clone(), w.clone()
+    table, n, out = table.to(dev), n.to(dev), out.to(dev)
+    kept, new = ops.kv_evict(k, v, table, n, w, budget, recent, sink=sink, out_tables=out)
+    for b in range(len(lens)):
+        assert int(new[b]) == min(lens[b], budget)
+        j = torch.arange(min(lens[b], budget), device=dev)
+        for h in range(hkv):
+            t = kept[b, h, :len(j)].long()
+            for now, before in ((k, k0), (v, v0)):
+                assert torch.equal(now[out[b, j // page].long(), h, j % page], before[table[b, t // page].long(), h, t % page])
+            assert torch.equal(w[b, h, :len(j)], w0[b, h, t])
+    if keeps == "all pages":  # the same as in place, wherever nothing was to be written too
+        k1, v1, w1 = k0.clone(), v0.clone(), w0.clone()
+        same, _ = ops.kv_evict(k1, v1, table, n, w1, budget, recent, sink=sink)
+        assert torch.equal(same, kept) and torch.equal(w, w1)
+        torch.testing.assert_close(k, k1, rtol=0, atol=0, equal_nan=True)
+        torch.testing.assert_close(v, v1, rtol=0, atol=0, equal_nan=True)
+
+
 def test_evict_bad_pages_and_lengths(dev):
     # rows on a page outside the cache are not moved; nothing else is touched
     q, k, v, table, n, g = _setup(4, torch.float16, [64], 1, 1, 64, 16)

@@ -10,7 +10,9 @@ is newer than them.
 ``csrc/bindings.cpp``, the extension module behind the decoding-step operators
 of ``ops``, is compiled with g++ against torch's headers into
 ``_bindings.so``; it reaches the kernels through the library that ``_lib``
-loads and links against torch alone.
+loads and links against torch alone. The library and the native harness need no
+torch: they are built also where the module cannot be, which is reported after
+them (without torch, a line on stderr; a failed compilation raises).
 
 Usage: ``python -m neso_b200.build [--force] [-v] [--ptxas-info]``
 """
@@ -71,7 +73,7 @@ def _compile(src: Path, force: bool, ptxas_info: bool) -> tuple[Path, str]:
 
 
 def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) -> Path:
-    """Compile every CUDA source for sm_100a and link ``libneso_b200.so``."""
+    """Compile every CUDA source for sm_100a, link ``libneso_b200.so`` and the harness, and build the extension module."""
     BUILD.mkdir(exist_ok=True)
     sources = sorted(CSRC.glob("*.cu"))
     if not sources:
@@ -79,7 +81,6 @@ def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) 
     with cf.ThreadPoolExecutor(max_workers=8) as ex:
         binding = ex.submit(build_binding, force)
         results = list(ex.map(lambda s: _compile(s, force, ptxas_info), sources))
-        binding.result()
     objs = [o for o, _ in results]
     if verbose or ptxas_info:
         for o, log in results:
@@ -93,14 +94,19 @@ def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) 
             raise RuntimeError(f"link failed:\n{' '.join(cmd)}\n{res.stdout}\n{res.stderr}")
         os.replace(tmp, LIB)
     build_harness(force)
+    binding.result()
     return LIB
 
 
-def build_binding(force: bool = False) -> Path:
-    """Compile the extension module against the installed torch."""
+def build_binding(force: bool = False) -> Path | None:
+    """Compile the extension module against the installed torch; None without one."""
     import sysconfig
 
-    import torch
+    try:
+        import torch
+    except ImportError as e:
+        print(f"{BINDING.name} is not built: {e}", file=sys.stderr)
+        return None
 
     root = Path(torch.__file__).resolve().parent
     newest = max(p.stat().st_mtime for p in (BINDING_SRC, root / "version.py", ROOT / "include" / "neso_b200.h"))

@@ -323,6 +323,45 @@ def test_attention_weights(dev, hq, hkv, D, window, extra, dtype):
         assert torch.equal(given[b, :, length:].cpu(), before[b, :, length:])
 
 
+BIAS = [(5.0, False, 0), (0.0, True, 0), (30.0, True, 50), (0.0, True, 37), (8.0, False, 100)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("softcap,use_slopes,window", BIAS)
+@pytest.mark.parametrize("D,hq,hkv,page", [(64, 12, 2, 16), (128, 8, 2, 24), (64, 24, 2, 8), (128, 12, 1, 16), (64, 20, 1, 16)])
+def test_attention_bias_over_runs(dev, D, hq, hkv, page, softcap, use_slopes, window, dtype):
+    # a table wide enough for runs, which pass from one ragged sequence to the next
+    q, k, v, table, n, g = _setup(hq + D, dtype, [200, 33, 1, 0, 700, 17, 90], hq, hkv, D, page, extra_width=16000 // page)
+    assert _lib.lib().neso_paged_attention_workspace(7, hq, hkv, D, table.shape[1], page, 0) > 0  # clusters need none
+    slopes = torch.rand(hq, generator=g) * 0.3 - 0.05 if use_slopes else None
+    _check_attention(q, k, v, table, n, D, dtype, softcap=softcap, slopes=slopes, window=window)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("softcap,use_slopes,window", BIAS)
+@pytest.mark.parametrize("D,hq,hkv,extra", [(64, 12, 2, 2), (128, 12, 1, 2), (64, 12, 2, 1000), (128, 8, 2, 1000), (64, 24, 2, 1000),
+                                            (128, 12, 1, 1000), (64, 20, 1, 1000)])  # 1000: a table for runs
+def test_attention_weights_of_biased_scores(dev, D, hq, hkv, extra, softcap, use_slopes, window, dtype):
+    lens = [0, 1, 31, 150, 700]
+    q, k, v, table, n, g = _setup(hq + D, dtype, lens, hq, hkv, D, 16, extra_width=extra)
+    slopes = torch.rand(hq, generator=g) * 0.3 - 0.05 if use_slopes else None
+    before = torch.rand(5, hkv, table.shape[1] * 16, generator=g)
+    after = torch.full_like(before, -1.0).cuda()
+    _, sums, tol = _check_attention(q, k, v, table, n, D, dtype, softcap=softcap, slopes=slopes, window=window,
+                                    weights=before.cuda(), weights_out=after)
+    for b, length in enumerate(lens):
+        for kv in range(hkv):
+            add = torch.zeros(before.shape[2], dtype=torch.float64)
+            for t, x in sums.get((b, kv), {}).items():
+                add[t] = x
+            want = before[b, kv].double() + add
+            # The sum takes the query heads one after the other: a rounding of at most U of it for
+            # each, hq / hkv in all, where a token's own share of the weight may be far smaller.
+            bound = tol * add + (hq // hkv + 1) * U * want + 2.0 ** -60
+            assert bool(((after[b, kv].cpu().double() - want).abs() <= bound)[:length].all())
+            assert bool((after[b, kv, length:] == -1.0).all())
+
+
 def test_attention_long_and_far(dev):
     # a cache of more than 2^32 elements, the sequences' pages at both ends; many runs per head are joined
     D, hkv, page, lens = 128, 8, 64, [20011, 37]

@@ -109,7 +109,9 @@ bool overlap(const at::Tensor& a, const at::Tensor& b) {
 // An output may be the input itself or must not touch it.
 void same_or_apart(const at::Tensor& a, const at::Tensor& b, const char* what) {
   if (!overlap(a, b)) return;
-  if (a.data_ptr() == b.data_ptr() && a.sizes() == b.sizes() && a.strides() == b.strides()) return;
+  bool same = a.data_ptr() == b.data_ptr() && a.sizes() == b.sizes();
+  for (int64_t i = 0; same && i < a.dim(); ++i) same = step_of(a, i) == step_of(b, i);
+  if (same) return;
   value_error(std::string(what) + " overlap without being the same tensor");
 }
 

@@ -870,6 +870,26 @@ def test_logits_strides_and_in_place(dev, dtype):
         assert bool((wide[:, :shift] == 0).all()) and bool((wide[:, shift + 9001:] == 0).all())
 
 
+def test_in_place_views_of_one_row_whose_batch_strides_differ(dev):
+    # the stride of a dimension of one has no meaning: these are the same tensor
+    x, kw = _logit_inputs(10, 1, 100, 20, torch.float32)
+    buf = torch.zeros(1, 128, device=dev)
+    view = buf[:, :100]
+    view.copy_(x)
+    same = view.as_strided((1, 100), (100, 1))
+    assert view.stride() != same.stride()
+    want = ops.process_logits(x.cuda(), **{k: t.cuda() for k, t in kw.items()})
+    assert _check_logits(x, kw, xd=view, out=same) is same and torch.equal(view, want)
+    q, k, v, table, n, g = _setup(24, torch.float16, [20], 4, 2, 64, 16)
+    w = torch.rand(2, 2, 50, generator=g).cuda()
+    one = w[:1, :, :32]
+    other = one.as_strided((1, 2, 32), (1, 50, 1))
+    before = one.clone()
+    ops.paged_attention(q, k, v, table.cuda(), n.cuda(), weights=one, weights_out=other)
+    ops.paged_attention(q, k, v, table.cuda(), n.cuda(), weights=before)
+    assert torch.equal(one, before)
+
+
 def test_logits_graph(dev):
     x, kw = _logit_inputs(9, 2, 4000, 50, torch.float32)
     kw = {k: v.cuda() for k, v in kw.items()}

@@ -84,11 +84,38 @@ void rows(const at::Tensor& t, const char* name) {
 // Stride of a dimension; 0 where its length leaves the stride without a meaning.
 int64_t step_of(const at::Tensor& t, int64_t dim) { return t.size(dim) > 1 ? t.stride(dim) : 0; }
 
-void written(const at::Tensor& t, const char* name) {
-  for (int64_t i = 0; i < t.dim(); ++i) {
-    if (t.size(i) > 1 && t.stride(i) == 0) {
-      value_error(std::string(name) + " is written to and must not be an expanded view");
+// The dimensions of `t` that are longer than one, the widest stride first.
+struct Dims {
+  int n = 0;
+  int64_t size[4], stride[4];
+};
+Dims dims_of(const at::Tensor& t) {
+  Dims d;
+  const at::IntArrayRef sizes = t.sizes(), strides = t.strides();
+  for (size_t i = 0; i < sizes.size(); ++i) {
+    if (sizes[i] <= 1) continue;
+    int at = d.n++;
+    for (; at > 0 && d.stride[at - 1] < strides[i]; --at) {
+      d.size[at] = d.size[at - 1];
+      d.stride[at] = d.stride[at - 1];
     }
+    d.size[at] = sizes[i];
+    d.stride[at] = strides[i];
+  }
+  return d;
+}
+
+// A tensor that is written to: each step of a dimension passes all that the
+// narrower dimensions hold, so that no two elements are one.
+void written(const at::Tensor& t, const char* name) {
+  if (t.numel() == 0) return;
+  const Dims d = dims_of(t);
+  int64_t span = 1;
+  for (int i = d.n - 1; i >= 0; --i) {
+    if (d.stride[i] < span) {
+      value_error(std::string(name) + " is written to and must not be an expanded view or overlap itself");
+    }
+    span += (d.size[i] - 1) * d.stride[i];
   }
 }
 
@@ -106,6 +133,41 @@ bool overlap(const at::Tensor& a, const at::Tensor& b) {
   const Extent x = extent(a), y = extent(b);
   return x.first < y.end && y.first < x.end;
 }
+// Whether elements [lo, hi) hold one of the view of dimensions i and on of d
+// that starts at 0.
+bool holds(const Dims& d, int i, int64_t lo, int64_t hi) {
+  if (hi <= 0) return false;
+  if (i == d.n) return lo <= 0;
+  int64_t span = 1;  // of one step
+  for (int j = i + 1; j < d.n; ++j) span += (d.size[j] - 1) * d.stride[j];
+  const int64_t step = d.stride[i];
+  if (step == 0) return holds(d, i + 1, lo, hi);
+  const int64_t first = lo < span ? 0 : (lo - span) / step + 1;  // the first step that ends behind lo
+  for (int64_t x = first; x < d.size[i] && x * step < hi; ++x) {
+    if (lo <= x * step && x * step < hi) return true;  // its first element
+    if (holds(d, i + 1, lo - x * step, hi - x * step)) return true;
+  }
+  return false;
+}
+
+// An output must not touch an input, None or a tensor, or a cache (which may
+// surround it: a buffer that holds pages and other things).
+void apart(const at::Tensor& out, const char* name, PyObject* other, const char* what) {
+  if (other == Py_None || !overlap(out, THPVariable_Unpack(other))) return;
+  value_error(std::string(name) + " overlaps " + what);
+}
+void apart(const at::Tensor& out, const char* name, const at::Tensor& cache, const char* what) {
+  if (!overlap(out, cache)) return;
+  const Extent x = extent(out);
+  const int64_t size = cache.element_size();
+  const int64_t lo = static_cast<int64_t>(x.first - reinterpret_cast<uintptr_t>(cache.data_ptr()));
+  const int64_t hi = static_cast<int64_t>(x.end - reinterpret_cast<uintptr_t>(cache.data_ptr()));
+  // Whole elements of the cache: floor and ceiling of bytes that may be negative.
+  if (holds(dims_of(cache), 0, lo >= 0 ? lo / size : -((-lo + size - 1) / size), hi >= 0 ? (hi + size - 1) / size : 0)) {
+    value_error(std::string(name) + " overlaps " + what);
+  }
+}
+
 // An output may be the input itself or must not touch it.
 void same_or_apart(const at::Tensor& a, const at::Tensor& b, const char* what) {
   if (!overlap(a, b)) return;
@@ -253,6 +315,10 @@ PyObject* rope_paged_append(PyObject* const* a) {
     out = cuda_tensor(a[10], "out", {q.scalar_type()}, 3, device);
     if (out.sizes() != q.sizes() || !out.is_contiguous()) value_error("out must be contiguous and of q's shape");
     same_or_apart(out, q, "out and q");
+    static const char* const names[9] = {"q", "k", "v", "cos", "sin", "positions", "slots", "k_cache", "v_cache"};
+    for (int i = 1; i < 7; ++i) apart(out, "out", a[i], names[i]);
+    apart(out, "out", c.k, names[7]);
+    apart(out, "out", c.v, names[8]);
   }
   const neso_stream_t stream = stream_on(device);
   const int rc = entry.rope_paged_append(
@@ -290,6 +356,12 @@ PyObject* paged_attention(PyObject* const* a) {
     const at::Tensor& wo = weights_of(wout, "weights_out", B, c.heads, tokens, device);
     same_or_apart(wo, wi, "weights and weights_out");
     written(wo, "weights_out");
+    apart(wo, "weights_out", a[0], "q");
+    apart(wo, "weights_out", c.k, "k_cache");
+    apart(wo, "weights_out", c.v, "v_cache");
+    apart(wo, "weights_out", a[3], "block_tables");
+    apart(wo, "weights_out", a[4], "seq_lens");
+    apart(wo, "weights_out", a[8], "slopes");
     for (int i = 0; i < 2; ++i) {
       win_s[i] = step_of(wi, i);
       wout_s[i] = step_of(wo, i);
@@ -304,6 +376,15 @@ PyObject* paged_attention(PyObject* const* a) {
     out = cuda_tensor(a[11], "out", {q.scalar_type()}, 3, device);
     if (out.sizes() != q.sizes() || !out.is_contiguous()) value_error("out must be contiguous and of q's shape");
     if (overlap(out, q)) value_error("out must not overlap q");
+    apart(out, "out", c.k, "k_cache");
+    apart(out, "out", c.v, "v_cache");
+    apart(out, "out", a[3], "block_tables");
+    apart(out, "out", a[4], "seq_lens");
+    apart(out, "out", a[8], "slopes");
+    if (weighted) {
+      apart(out, "out", a[9], "weights");
+      apart(out, "out", wout, "weights_out");
+    }
   }
   const neso_stream_t stream = stream_on(device);
   const int32_t b32 = size32(B, "B"), hq32 = size32(hq, "Hq"), width = static_cast<int32_t>(tables.size(1));
@@ -344,6 +425,11 @@ PyObject* kv_evict(PyObject* const* a) {
   written(c.k, "k_cache");
   written(c.v, "v_cache");
   written(wo, "weights_out");
+  apart(wo, "weights_out", c.k, "k_cache");
+  apart(wo, "weights_out", c.v, "v_cache");
+  apart(wo, "weights_out", a[2], "block_tables");
+  apart(wo, "weights_out", a[3], "seq_lens");
+  apart(wo, "weights_out", a[8], "out_tables");
   at::Tensor kept = empty({B, c.heads, budget > 0 ? budget : 0}, at::kInt, device);
   at::Tensor new_lens = empty({B}, at::kInt, device);
   const neso_stream_t stream = stream_on(device);
@@ -414,6 +500,9 @@ PyObject* process_logits(PyObject* const* a) {
     if (out.sizes() != x.sizes()) value_error("out must have the shape of logits");
     same_or_apart(out, x, "out and logits");
     written(out, "out");
+    static const char* const inputs[9] = {"history",  "history_lens", "prompt_lens", "repetition", "frequency",
+                                          "presence", "bias_ids",     "bias",        "mask"};
+    for (int i = 0; i < 9; ++i) apart(out, "out", a[1 + i], inputs[i]);
   }
   const neso_stream_t stream = stream_on(device);
   const int rc = entry.process_logits(

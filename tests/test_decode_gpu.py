@@ -928,6 +928,80 @@ def test_logits_refusals(dev):
         ops.process_logits(big[:, :100], out=big[:, 1:101])
 
 
+def test_outputs_that_touch_other_inputs_are_refused(dev):
+    q, k, v, table, n, g = _setup(25, torch.float16, [20, 3], 8, 2, 64, 16)
+    table, n = table.to(dev), n.to(dev)
+    slopes = torch.zeros(8, device=dev)
+    w = torch.zeros(2, 2, 40, device=dev)
+    page = k.flatten()[:1024].view(2, 8, 64)  # the output's shape, over the cache
+    far = v.flatten()[-1024:].view(2, 8, 64)
+    attend = ops.paged_attention
+    for out in (page, far):
+        with pytest.raises(ValueError, match="out overlaps [kv]_cache"):
+            attend(q, k, v, table, n, out=out)
+    big = torch.zeros(4096, device=dev)  # 32-bit words seen as other things
+    half = big.view(torch.float16)[:1024].view(2, 8, 64)
+    for name, kw in (("slopes", dict(slopes=big[500:508])), ("weights", dict(weights=big[100:260].view(2, 2, 40), weights_out=w))):
+        with pytest.raises(ValueError, match=f"out overlaps {name}"):
+            attend(q, k, v, table, n, out=half, **kw)
+    with pytest.raises(ValueError, match="out overlaps block_tables"):
+        attend(q, k, v, big.view(torch.int32)[:4].view(2, 2), n, out=half)
+    with pytest.raises(ValueError, match="weights_out overlaps q"):
+        attend(half, k, v, table, n, weights=w, weights_out=big[300:460].view(2, 2, 40))
+    with pytest.raises(ValueError, match="weights_out overlaps k_cache"):
+        kb = big.view(torch.float16)[:8192].view(4, 2, 16, 64)
+        attend(q, kb, kb.clone(), table, n, weights=w, weights_out=big[300:460].view(2, 2, 40))
+    with pytest.raises(ValueError, match="weights_out overlaps v_cache"):
+        ops.kv_evict(kb.clone(), kb, table, n, w, 8, 2, weights_out=big[300:460].view(2, 2, 40))
+    with pytest.raises(ValueError, match="overlap itself"):
+        ops.kv_evict(k, v, table, n, w, 8, 2, weights_out=torch.zeros(200, device=dev).as_strided((2, 2, 40), (40, 20, 1)))
+    with pytest.raises(ValueError, match="overlap itself"):
+        ops.kv_evict(k.as_strided(k.shape, (1024, 512, 64, 1)), v, table, n, w, 8, 2)
+    cos, pos, slots = torch.zeros(10, 32, device=dev), torch.zeros(2, dtype=torch.int32, device=dev), torch.arange(2, device=dev)
+    new = torch.zeros(2, 8 * 64 + 2 * 2 * 64, dtype=torch.float16, device=dev)
+    nk, nv = new[:, 512:640].view(2, 2, 64), new[:, 640:].view(2, 2, 64)
+    append = ops.rope_paged_append
+    for out, name in ((page, "k_cache"), (far, "v_cache"), (new.flatten()[:1024].view(2, 8, 64), "k")):
+        with pytest.raises(ValueError, match=f"out overlaps {name}"):
+            append(q, nk, nv, cos, cos, pos, slots, k, v, out=out)
+    with pytest.raises(ValueError, match="out overlaps sin"):
+        append(q, nk, nv, cos, big[:320].view(10, 32), pos, slots, k, v, out=half)
+    x = torch.zeros(2, 100, device=dev)
+    out = big[:200].view(2, 100)
+    ids = big.view(torch.int32)[:6].view(2, 3)
+    some = torch.zeros(2, dtype=torch.int32, device=dev)
+    for name, kw in (("history", dict(history=ids, history_lens=some)), ("mask", dict(mask=big.view(torch.int32)[:8].view(2, 4))),
+                     ("bias", dict(bias_ids=ids.clone(), bias=big[190:196].view(2, 3))),
+                     ("presence", dict(history=ids.clone(), history_lens=some, presence=big[199:201]))):
+        with pytest.raises(ValueError, match=f"out overlaps {name}"):
+            ops.process_logits(x, out=out, **kw)
+    with pytest.raises(ValueError, match="overlap itself"):
+        ops.process_logits(x, out=big[:200].as_strided((2, 100), (60, 1)))
+
+
+def test_outputs_between_the_pages_of_a_buffer(dev):
+    # pages and other things in one buffer: an output in the room that the pages leave is apart from them
+    q, k, v, table, n, g = _setup(26, torch.float16, [40, 3], 8, 2, 64, 16)
+    buf = torch.zeros(k.shape[0], 2 * 2048 + 1024 + 256, dtype=torch.float16, device=dev)
+    kb, vb = (buf[:, i * 2048:(i + 1) * 2048].view(-1, 2, 16, 64) for i in range(2))
+    kb.copy_(k), vb.copy_(v)
+    out = buf[1, 4096:5120].view(2, 8, 64)
+    w = buf.view(torch.float32)[2, 2560:2688].view(2, 2, 32)
+    w2 = torch.zeros(2, 2, 48, device=dev)
+    table, n = table.to(dev), n.to(dev)
+    assert ops.paged_attention(q, kb, vb, table, n, weights=w2, out=out) is out
+    assert torch.equal(out, ops.paged_attention(q, k, v, table, n))
+    short = torch.tensor([16, 3], dtype=torch.int32, device=dev)
+    w.zero_()
+    ops.kv_evict(kb, vb, table[:, :2], short, w2[:, :, :32], 4, 2, weights_out=w)
+    assert torch.equal(out, ops.paged_attention(q, k, v, table, n)) and float(w[0].abs().sum()) > 0
+    # heads that share one key: a view with a stride of 0 is read, beside a given output
+    one, val = k[:, :1].expand(-1, 2, -1, -1), v[:, :1].expand(-1, 2, -1, -1)
+    given = torch.empty_like(q)
+    ops.paged_attention(q, one, val, table, n, out=given)
+    assert torch.equal(given, ops.paged_attention(q, one.contiguous(), val.contiguous(), table, n))
+
+
 # ------------------------------------------------------ torch operators ----
 def test_torch_operators_match_tensor_api(dev):
     import neso_b200.torch_ops  # noqa: F401

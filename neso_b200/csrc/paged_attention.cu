@@ -40,6 +40,9 @@
 // that end between 82 and 98 us because SMs reach memory at different rates.
 #include <cooperative_groups.h>
 
+#include <map>
+#include <mutex>
+
 #include "paged.h"
 
 namespace neso {
@@ -1026,6 +1029,54 @@ constexpr int kSegTokens = 1024;
 // A CTA is worth having for this many tokens.
 constexpr int kSegLeast = 128;
 
+void cluster_launch(cudaLaunchConfig_t* cfg, cudaLaunchAttribute (&attr)[2], int clusters, int size, int smem,
+                    cudaStream_t stream) {
+  *cfg = cudaLaunchConfig_t{};
+  cfg->gridDim = dim3(static_cast<unsigned>(clusters * size));
+  cfg->blockDim = dim3(kSegThreads);
+  cfg->dynamicSmemBytes = smem;
+  cfg->stream = stream;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(size);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg->attrs = attr;
+  cfg->numAttrs = 2;
+}
+
+// Whether the current device can hold a cluster of sixteen, which is more than
+// every device has to (asked once, of the variant that needs most; without a
+// device, the B200's answer).
+template <int D>
+bool holds_big_cluster() {
+  static std::mutex mu;
+  static std::map<int, bool> known;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) {
+    cudaGetLastError();
+    return true;
+  }
+  std::lock_guard<std::mutex> lock(mu);
+  const auto it = known.find(dev);
+  if (it != known.end()) return it->second;
+  constexpr int smem = kSegWarps * Warp<true, D, 2, true, true>::kRing;
+  auto* kern = paged_attention_segment_kernel<true, D, 2, true, true>;
+  cudaLaunchConfig_t cfg;
+  cudaLaunchAttribute attr[2];
+  cluster_launch(&cfg, attr, 1, kBigCluster, smem, nullptr);
+  cfg.numAttrs = 1;  // the cluster's size
+  int most = 0;
+  if (kernel_setup(reinterpret_cast<const void*>(kern), smem, nullptr) != NESO_OK ||
+      cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&most, kern, &cfg) != cudaSuccess) {
+    cudaGetLastError();
+    most = 0;
+  }
+  return known[dev] = most > 0;
+}
+
 struct Plan {
   int group, tiles, rows, nt, ctas, warps;
   int64_t capacity;
@@ -1056,7 +1107,8 @@ int make_plan(int B, int hq, int hkv, int D, int width, int page_size, bool weig
   }
   pl.cluster = 1;
   while (pl.cluster < kMaxCluster && segments * pl.cluster * 2 <= sm_count() && pl.cluster * kSegLeast < pl.capacity) pl.cluster *= 2;
-  if (pl.cluster == kMaxCluster && pl.cluster * kSegLeast < pl.capacity && segments * kBigCluster * (D == 64 ? 1 : 2) <= sm_count()) {
+  if (pl.cluster == kMaxCluster && pl.cluster * kSegLeast < pl.capacity &&
+      segments * kBigCluster * (D == 64 ? 1 : 2) <= sm_count() && (D == 64 ? holds_big_cluster<64>() : holds_big_cluster<128>())) {
     pl.cluster = kBigCluster;
   }
   pl.by_segment = segments <= sm_count() * (D == 64 ? 2 : 1) && pl.tiles == 1 &&
@@ -1097,20 +1149,9 @@ int launch_attention(const AttnParams& p, const Plan& pl, cudaStream_t stream) {
       const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
       if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute");
     }
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(p.B * p.hkv * pl.cluster));
-    cfg.blockDim = dim3(kSegThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
+    cudaLaunchConfig_t cfg;
     cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = static_cast<unsigned>(pl.cluster);
-    attr[1].val.clusterDim.y = 1;
-    attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 2;
+    cluster_launch(&cfg, attr, p.B * p.hkv, pl.cluster, smem, stream);
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
     return e == cudaSuccess ? ok() : cuda_fail(e, "paged_attention launch");
   }

@@ -121,6 +121,16 @@ def test_attention_shapes(dev, case, dtype):
     _check_attention(q, k, v, table, n, D, dtype)
 
 
+def test_attention_clusters_of_sixteen_are_found(dev):
+    # very few pairs whose tables are too long for eight CTAs take sixteen, without a workspace,
+    # where the device can hold such a cluster, and the workspace follows what the call then does
+    need = _lib.lib().neso_paged_attention_workspace
+    _lib.lib().neso_set_device(0)
+    assert need(1, 3, 1, 64, 1000, 16, 0) == 0 and need(1, 16, 1, 128, 512, 16, 0) == 0
+    assert need(1, 3, 1, 64, 1025, 16, 0) > 0 and need(8, 16, 1, 128, 1000, 16, 0) > 0
+    assert _lib.last_error() == ""
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("window", [1, 15, 16, 17, 100])
 def test_attention_window(dev, window, dtype):

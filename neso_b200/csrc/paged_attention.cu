@@ -54,9 +54,10 @@ constexpr int kUnit = 16;      // tokens per unit
 constexpr int kStages = 3;     // units in flight per warp
 constexpr int kWarps = 4;      // warps per CTA
 constexpr int kThreads = kWarps * 32;
-// Cost of starting a segment, in units (64 ragged sequences: 77.6 us; 86.7 with
-// 0, 76.5 with 2, 78.3 with 8).
-constexpr int kStart = 4;
+// Cost of starting a segment, in units. With 0 / 1 / 2 / 4 / 8: 64 ragged sequences
+// 85.6 / 76.5 / 76.8 / 76.8 / 76.7 us, 48 sequences under a window 25.8 / 25.1 / 25.1 /
+// 25.5 / 26.3, 256 sequences of 500 tokens 98.3 / 95.3 / 97.0 / 99.1 / 97.2.
+constexpr int kStart = 1;
 // Least points of a run: shorter ones leave more pieces to join, longer ones
 // fewer warps (2048 tokens as runs: 10.7 us with 2, 10.6 with 4, 14.3 with 6).
 constexpr int kMinRun = 4;

@@ -26,7 +26,6 @@ namespace {
 constexpr int kLong = 24, kLongThreads = 512;
 constexpr int kShortThreads = 256;
 constexpr int kMostThreads = 1024;  // per SM
-constexpr int kEarly = 1;  // fours of history tokens per thread and round
 // A count word: generated occurrences, and two flags.
 constexpr uint32_t kSeen = 0x80000000u;    // the token occurs in the history
 constexpr uint32_t kBiased = 0x40000000u;  // the token has a bias
@@ -136,13 +135,12 @@ __global__ void __launch_bounds__(kThreads, kMostThreads / kThreads)
 
   // Requests.
   int n = 0, prompt = 0;
-  int4 id[kEarly];
+  int4 id;  // four of the history's tokens
   const int32_t* ids = p.history + b * p.history_stride;
   if (p.history != nullptr) {
     n = p.history_lens[b];
     if (p.prompt_lens != nullptr) prompt = p.prompt_lens[b];
-#pragma unroll
-    for (int j = 0; j < kEarly; ++j) id[j] = load_four(ids, tid + j * kThreads, p.T);
+    id = load_four(ids, tid, p.T);
   }
   const int32_t* bias_ids = p.bias_ids + static_cast<int64_t>(b) * p.num_bias;
   const float* bias = p.bias + static_cast<int64_t>(b) * p.num_bias;
@@ -187,14 +185,9 @@ __global__ void __launch_bounds__(kThreads, kMostThreads / kThreads)
         }
       }
     };
-    for (int i = tid; 4 * i < n;) {
-#pragma unroll
-      for (int j = 0; j < kEarly; ++j) count(id[j], i + j * kThreads);
-      i += kEarly * kThreads;
-      if (4 * i < n) {
-#pragma unroll
-        for (int j = 0; j < kEarly; ++j) id[j] = load_four(ids, i + j * kThreads, p.T);
-      }
+    for (int i = tid; 4 * i < n; i += kThreads) {
+      if (i != tid) id = load_four(ids, i, p.T);
+      count(id, i);
     }
   }
   for (int i = tid; i < p.num_bias; i += kThreads) {

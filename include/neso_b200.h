@@ -334,7 +334,10 @@ NESO_API int neso_rope_paged_append(const void* q, const void* k, const void* v,
  * weights_out[b, kv, t] = weights_in[b, kv, t] + the sum of the softmax
  * weights of the kv head's query heads, for t < seq_lens[b]; the rest is left.
  * A length is clamped to [0, table_width * page_size]; tokens of a page
- * outside [0, num_pages) are left out; with no token left the row is zero. */
+ * outside [0, num_pages) are left out, as is one whose score is -inf; with no
+ * token left the row is zero. Distances (slopes, window) count cached tokens:
+ * after neso_kv_evict has closed the gaps, they are distances in the trimmed
+ * cache, not between the positions that the keys were rotated by. */
 NESO_API int neso_paged_attention(const void* q, const void* k_cache, const void* v_cache,
                                   const int32_t* block_tables, const int32_t* seq_lens, const float* slopes,
                                   const float* weights_in, float* weights_out, void* out, void* workspace,

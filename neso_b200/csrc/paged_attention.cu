@@ -8,9 +8,10 @@
 //   weights_out[b, kv, t] = weights_in[b, kv, t] + sum over the kv head's
 //             query heads of p[h, t]                   if weights are given
 //
-// Every visible key and value is read once for all the query heads of its kv
-// head: 4 D bytes per token and kv head against 4 D FLOP per token and query
-// head, far below the tensor cores' ridge, so HBM bounds it.
+// Every visible key and value is read once for up to 16 query heads of its kv
+// head (larger groups in several passes): 4 D bytes per token and kv head against
+// 4 D FLOP per token and query head, far below the tensor cores' ridge, so HBM
+// bounds it.
 //
 // Work: the cache is cut into units of 16 tokens of one (sequence, kv head).
 // All units of the batch, in order, are dealt out in equal contiguous runs to
@@ -33,11 +34,12 @@
 // fp16: 2^-22, see kParts and kRaise), so the output's own rounding is what
 // remains; the tensor cores are idle enough to do it several times.
 //
-// Measured (B200, D = 128): one sequence of 131071 tokens, 32 / 8 heads, 93 us =
+// Measured (B200, D = 128): one sequence of 131071 tokens, 32 / 8 heads, 92.5 us =
 // 5.8 TB/s of keys and values, 88 % of the rate of a large copy; 64 ragged
-// sequences of 5 to 8192 tokens, 64 / 8 heads, 74.5 us = 5.6 TB/s. What is
+// sequences of 5 to 8192 tokens, 64 / 8 heads, 75 us = 5.5 TB/s. What is
 // missing: 5 us until the first keys arrive, the join (4 us), and equal runs
-// that end between 82 and 98 us because SMs reach memory at different rates.
+// that end at different times, because SMs reach memory at different rates (the
+// last 16 us after the first in a run slowed by time stamps).
 #include <cooperative_groups.h>
 
 #include <map>
@@ -59,7 +61,8 @@ constexpr int kThreads = kWarps * 32;
 // 25.5 / 26.3, 256 sequences of 500 tokens 98.3 / 95.3 / 97.0 / 99.1 / 97.2.
 constexpr int kStart = 1;
 // Least points of a run: shorter ones leave more pieces to join, longer ones
-// fewer warps (2048 tokens as runs: 10.7 us with 2, 10.6 with 4, 14.3 with 6).
+// fewer warps (8192 tokens of 16 / 1 heads as runs: 15.4 us with 2, 13.6 with 4, 15.8
+// with 6; 2048 of 32 / 8: 11.2, 11.2, 14.4).
 constexpr int kMinRun = 4;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -646,8 +649,8 @@ constexpr int kSegThreads = kSegWarps * 32;
 constexpr int kMaxCluster = 8;
 // Very few pairs: clusters of this size, which a GPC of the B200 still holds (a
 // CTA to an SM at D = 128, so that only half the SMs are counted on). One
-// sequence of 8192 tokens: 16 / 1 heads x 128 18.5 -> 12.9 us, 32 / 8 x 64
-// 12.2 -> 9.9; 32 / 8 x 128 would take 20.2 instead of 14.9, as the eight
+// sequence of 8192 tokens: 16 / 1 heads x 128 17.8 -> 12.5 us, 32 / 8 x 64
+// 11.9 -> 9.8; 32 / 8 x 128 would take 20.1 instead of 14.7, as the eight
 // clusters are not on the SMs together.
 constexpr int kBigCluster = 16;
 
@@ -1022,13 +1025,13 @@ __global__ void __launch_bounds__(kJoinThreads, kScores ? 4 : 2) paged_attention
 }
 
 // A cluster per (sequence, kv head) where the clusters fit the SMs (two CTAs each
-// at D = 64: 256 pairs of up to 300 tokens 7.0 us, as runs 11.6; at D = 128 one:
-// 160 pairs of 900 tokens 22.1 us so, 20.0 as runs) and the tables hold at most
+// at D = 64: 256 pairs of up to 300 tokens 7.3 us, as runs 12.2; at D = 128 one:
+// 160 pairs of up to 900 tokens 17.2 us so, 16.6 as runs) and the tables hold at most
 // kSegTokens tokens per CTA. One sequence, 32 / 8 heads,
-// D = 128, 512 / 1024 / 2048 / 8192 tokens: 5.9 / 6.7 / 8.1 / 14.7 us so,
-// 10.2 / 11.7 / 10.5 / 15.8 us as runs; beyond, the few CTAs' share of the
-// bandwidth falls behind (8 pairs of up to 9000 tokens: 19.6 against 16.5 us; at
-// D = 128 and 16 CTAs beyond half of that, 16384 tokens: 19.0 against 17.0).
+// D = 128, 512 / 1024 / 2048 / 8192 tokens: 6.1 / 6.7 / 8.2 / 14.7 us so,
+// 10.9 / 13.3 / 11.2 / 16.4 us as runs; beyond, the few CTAs' share of the
+// bandwidth falls behind (8 pairs of up to 9000 tokens: 19.2 against 16.8 us; at
+// D = 128 and 16 CTAs beyond half of that, 16384 tokens: 18.0 against 17.2).
 constexpr int kSegTokens = 1024;
 // A CTA is worth having for this many tokens.
 constexpr int kSegLeast = 128;

@@ -17,8 +17,9 @@
 // so when all rows of a step are in shared memory (a cluster barrier), the rows
 // that it overwrites are not the source of any later step, and later steps may
 // already be on their way in. 8 sequences x 8 heads of up to 4096 tokens to
-// 2048, D = 128: 34.5 us under a table of their own, of which the rows take 22.3
-// (6 TB/s read and written, as a plain copy) and the selection the rest.
+// 2048, D = 128: 34.3 us under a table of their own, of which the rows take 22.3
+// (6 TB/s read and written, as a plain copy) and the selection the rest; 44.1 in
+// place, a cluster barrier per step.
 #include <cooperative_groups.h>
 
 #include "paged.h"
@@ -637,7 +638,8 @@ constexpr int kApartLoads = 4;
 // of the block table, or a table that keeps some pages) has rows that are a source
 // for one move and the end of another. One CTA moves all of them then, in order: the
 // rows of a step are all loaded before the first is stored, and later steps read
-// behind the rows that it stores.
+// behind the rows that it stores. The case above takes 180 us so, 44 where the
+// caller says that it is in place.
 __device__ __forceinline__ void move_ordered(const EvictParams& p, int b, int h, int keep, const int32_t* kept) {
   constexpr int kThreads = kApartWarps * 32;
   const int pieces = p.D / 8, row_items = 2 * pieces;

@@ -195,7 +195,9 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     query heads added, in place or into ``weights_out``, for t < len.
 
     Lengths are clamped to [0, width * page_size]; tokens of a page outside the
-    cache are left out; a sequence without tokens gives zeros."""
+    cache are left out; a sequence without tokens gives zeros. ``slopes`` and
+    ``window`` count cached tokens: after ``kv_evict`` these are distances in the
+    trimmed cache, not between the positions that the keys were rotated by."""
     return (_binding or _load_binding()).paged_attention(q, k_cache, v_cache, block_tables, seq_lens, scale, softcap, window,
                                                        slopes, weights, weights_out, out)
 
